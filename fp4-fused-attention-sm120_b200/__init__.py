@@ -21,12 +21,14 @@ __all__ = [
     "selftest_timeout", "selftest_abort", "supported_head_dims", "prepare", "attend", "shard_range", "SCALE_REFERENCE", "SCALE_OCP",
     "F32", "F16", "MASK_NONE", "MASK_CAUSAL", "fused_fp4_attention_lse", "backward_workspace_size",
     "fp4_attention_backward", "FP4Attention", "fp4_attention", "selftest_backward_abort",
+    "rotary_frequencies", "rotary_table", "rotary", "rotary_embedding", "PagedCache", "cache_append", "cache_gather",
+    "paged_attention_workspace_size", "paged_attention", "paged_attention_lse", "copy_pages", "PagePool",
 ]
 
 BLOCK_ELEMENT = 32  # common.h:15
 BQ = 64             # common.h:18
 
-OK, EINVAL, EUNSUPPORTED, ECUDA, ETIMEOUT, EWORKSPACE = range(6)
+OK, EINVAL, EUNSUPPORTED, ECUDA, ETIMEOUT, EWORKSPACE, EINDEX = range(7)
 F32, F16 = 0, 1
 SCALE_REFERENCE, SCALE_OCP = 0, 1
 LAYOUT_ROWMAJOR = 0
@@ -105,6 +107,7 @@ def lib() -> ctypes.CDLL:
     L.fp4attn_last_error.restype = ctypes.c_char_p
     L.fp4attn_supported_head_dims.argtypes = [ctypes.POINTER(i32), i32]
     L.fp4attn_supported_head_dims.restype = i32
+    _serving.declare(L)
     _LIB = L
     return L
 
@@ -416,3 +419,9 @@ def selftest_timeout(timeout_us: int = 2000, stream=None) -> int:
     """Run the bounded-wait expiry test kernel; returns status_query()."""
     _check(lib().fp4attn_selftest_timeout(timeout_us, _stream_ptr(stream)), "fp4attn_selftest_timeout")
     return status_query(stream)
+
+
+from . import _serving  # noqa: E402  (the serving modules use the helpers above)
+from .paged import (PagedCache, PagePool, cache_append, cache_gather, copy_pages, paged_attention,  # noqa: E402
+                    paged_attention_lse, paged_attention_workspace_size)
+from .rotary import rotary, rotary_embedding, rotary_frequencies, rotary_table  # noqa: E402

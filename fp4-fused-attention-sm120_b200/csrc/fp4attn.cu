@@ -791,9 +791,11 @@ namespace fp4attn {
 void set_error_detail(const char* msg) { g_last_error = msg; }
 
 // The host helpers above, for the library's other translation units
-// (backward.cu).
+// (backward_api.cuh, paged.cu).
 namespace host {
+int serving_status();  // paged.cu
 int error(int code, const char* msg) { return fail(code, "%s", msg); }
+void clear_error() { g_last_error.clear(); }
 int ready() { return device_ready(); }
 int sms() { return device_sms(); }
 unsigned long long timeout_ns() { return wait_timeout_ns(); }
@@ -968,7 +970,7 @@ int fp4attn_status_query(void* stream)
     FP4_CUDA(cudaStreamSynchronize(st));
     int host[4] = {0, 0, 0, 0};
     FP4_CUDA(cudaMemcpyFromSymbol(host, fp4attn::g_fp4attn_error, sizeof host));
-    if (host[0] == 0) return FP4ATTN_OK;
+    if (host[0] == 0) return fp4attn::host::serving_status();
     const int zero[4] = {0, 0, 0, 0};
     FP4_CUDA(cudaMemcpyToSymbol(fp4attn::g_fp4attn_error, zero, sizeof zero));
     return fail(host[0], "device wait expired at site %d (block %d,%d)", host[1], host[2], host[3]);
@@ -1018,6 +1020,7 @@ const char* fp4attn_error_string(int status)
         case FP4ATTN_ECUDA: return "CUDA error";
         case FP4ATTN_ETIMEOUT: return "device wait timed out";
         case FP4ATTN_EWORKSPACE: return "workspace missing or too small";
+        case FP4ATTN_EINDEX: return "index read on the device out of range";
     }
     return "unknown status";
 }

@@ -1,0 +1,409 @@
+// paged.cu -- the serving half of the C ABI (declared in include/fp4attn.h):
+// rotary positions, the paged cache and the attention over it.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "../../include/fp4attn.h"
+#include "paged.cuh"
+#include "paged_attention.cuh"
+#include "rotary.cuh"
+
+namespace fp4attn {
+namespace host {  // fp4attn.cu
+int error(int code, const char* msg);
+void clear_error();
+int ready();
+int sms();
+unsigned long long timeout_ns();
+
+// The serving kernels' error word, read and cleared (for fp4attn_status_query).
+int serving_status()
+{
+    int w[4] = {0, 0, 0, 0};
+    cudaError_t e = cudaMemcpyFromSymbol(w, g_serving_error, sizeof w);
+    if (e != cudaSuccess) return error(FP4ATTN_ECUDA, cudaGetErrorString(e));
+    if (w[0] == 0) return FP4ATTN_OK;
+    const int zero[4] = {0, 0, 0, 0};
+    e = cudaMemcpyToSymbol(g_serving_error, zero, sizeof zero);
+    if (e != cudaSuccess) return error(FP4ATTN_ECUDA, cudaGetErrorString(e));
+    char buf[160];
+    if (w[0] == FP4ATTN_EINDEX) {
+        static const char* const kinds[] = {"index", "position", "page", "sequence", "length or position"};
+        const long long value = (static_cast<long long>(w[3]) << 32) | static_cast<unsigned>(w[2]);
+        snprintf(buf, sizeof buf, "%s %lld out of range", kinds[w[1] >= 1 && w[1] <= 4 ? w[1] : 0], value);
+    } else {
+        snprintf(buf, sizeof buf, "device wait expired at serving site %d (block %d)", w[1], w[2]);
+    }
+    return error(w[0], buf);
+}
+}  // namespace host
+}  // namespace fp4attn
+
+namespace {
+
+using namespace fp4attn;
+
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int fail(int code, const char* fmt, ...)
+{
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return host::error(code, buf);
+}
+
+#define PAGED_CUDA(call)                                                                            \
+    do {                                                                                            \
+        cudaError_t e_ = (call);                                                                    \
+        if (e_ != cudaSuccess) return fail(FP4ATTN_ECUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
+    } while (0)
+
+bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool bad_dtype(int t) { return t != FP4ATTN_F32 && t != FP4ATTN_F16; }
+int bytes_of(int dtype) { return dtype == FP4ATTN_F16 ? 2 : 4; }
+bool supported_dim(int d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 160 || d == 256; }
+
+int check_cache(const fp4attn_cache* c)
+{
+    if (!c || !c->k_codes || !c->k_scales || !c->v) return fail(FP4ATTN_EINVAL, "null cache pointer");
+    if (!supported_dim(c->head_dim))
+        return fail(FP4ATTN_EUNSUPPORTED, "head_dim %d is not one of 32/64/96/128/160/256", c->head_dim);
+    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+        return fail(FP4ATTN_EUNSUPPORTED, "page_size %d is not one of 16/32/64/128", c->page_size);
+    if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 65535)
+        return fail(FP4ATTN_EINVAL, "pages %d >= 1, kv_heads %d in [1, 65535]", c->pages, c->kv_heads);
+    const int64_t rows = static_cast<int64_t>(c->kv_heads) * c->page_size;
+    if (rows * c->head_dim * 2 > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "a page of 2 GiB or more");
+    if (c->k_codes_stride < rows * c->head_dim / 2 || c->k_scales_stride < rows * c->head_dim / 32 ||
+        c->v_stride < rows * c->head_dim * 2)
+        return fail(FP4ATTN_EINVAL, "page strides smaller than a page");
+    if (!aligned(c->k_codes, 16) || !aligned(c->k_scales, 16) || !aligned(c->v, 16) ||
+        ((c->k_codes_stride | c->k_scales_stride | c->v_stride) & 15))
+        return fail(FP4ATTN_EINVAL, "cache pointers and page strides must be multiples of 16 bytes");
+    return FP4ATTN_OK;
+}
+
+int check_table(const int32_t* block_table, int64_t stride, int seqs, int max_pages)
+{
+    if (!block_table && seqs != 0) return fail(FP4ATTN_EINVAL, "null block table");
+    if (seqs < 0 || max_pages < 1 || stride < 0 || (seqs > 1 && stride < max_pages))
+        return fail(FP4ATTN_EINVAL, "block table of %d sequences, %d pages, stride %lld", seqs, max_pages,
+                    static_cast<long long>(stride));
+    return FP4ATTN_OK;
+}
+
+CacheView view_of(const fp4attn_cache& c)
+{
+    CacheView v{c.k_codes, c.k_scales, static_cast<__half*>(c.v), c.k_codes_stride, c.k_scales_stride, c.v_stride,
+                c.pages, c.page_size, 0, c.kv_heads, c.head_dim};
+    while ((1 << v.page_shift) < c.page_size) v.page_shift++;
+    return v;
+}
+
+int check_rotary(const float* table, int rotary_dim, int64_t max_positions, int head_dim)
+{
+    if (!table || !aligned(table, 16)) return fail(FP4ATTN_EINVAL, "the rotary table must be a 16-byte aligned pointer");
+    if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim)
+        return fail(FP4ATTN_EINVAL, "rotary_dim %d must be even, in [2, head_dim %d]", rotary_dim, head_dim);
+    if (max_positions < 1) return fail(FP4ATTN_EINVAL, "max_positions must be >= 1");
+    return FP4ATTN_OK;
+}
+
+// Whether rows at these strides take 16-byte accesses.
+bool wide(const void* p, int dtype, std::initializer_list<int64_t> strides)
+{
+    const int e = 16 / bytes_of(dtype);
+    if (!aligned(p, 16)) return false;
+    for (int64_t s : strides)
+        if (s % e) return false;
+    return true;
+}
+
+// Whether eights of a row are turned whole: the rotated part (halves: each
+// half of it) is a multiple of eight elements.
+bool whole_eights(int rot, int interleaved) { return (interleaved ? rot : rot / 2) % 8 == 0; }
+
+template <typename T>
+void launch_rotary(dim3 grid, cudaStream_t st, const RotaryArgs& a, bool vec, bool inter)
+{
+    if (vec && inter) rotary_kernel<T, true, true><<<grid, 256, 0, st>>>(a);
+    else if (vec) rotary_kernel<T, true, false><<<grid, 256, 0, st>>>(a);
+    else if (inter) rotary_kernel<T, false, true><<<grid, 256, 0, st>>>(a);
+    else rotary_kernel<T, false, false><<<grid, 256, 0, st>>>(a);
+}
+
+template <typename InT, typename OutT>
+int launch_attention(const PagedArgs& a, cudaStream_t st)
+{
+    const dim3 grid(a.q_heads, a.batch);
+    switch (a.c.head_dim) {
+        case 32: paged_attention_simple_kernel<InT, OutT, 32><<<grid, 128, 0, st>>>(a); break;
+        case 64: paged_attention_simple_kernel<InT, OutT, 64><<<grid, 128, 0, st>>>(a); break;
+        case 96: paged_attention_simple_kernel<InT, OutT, 96><<<grid, 128, 0, st>>>(a); break;
+        case 128: paged_attention_simple_kernel<InT, OutT, 128><<<grid, 128, 0, st>>>(a); break;
+        case 160: paged_attention_simple_kernel<InT, OutT, 160><<<grid, 128, 0, st>>>(a); break;
+        default: paged_attention_simple_kernel<InT, OutT, 256><<<grid, 128, 0, st>>>(a); break;
+    }
+    PAGED_CUDA(cudaGetLastError());
+    return FP4ATTN_OK;
+}
+
+template <int kArrays, int kPairs>
+int launch_copies(const std::vector<CopyArray>& arrays, const int32_t* src, const int32_t* dst, int n, cudaStream_t st)
+{
+    CopyArgs<kArrays, kPairs> a;
+    for (size_t first = 0; first < arrays.size(); first += kArrays) {
+        a.n_arrays = static_cast<int>(std::min<size_t>(kArrays, arrays.size() - first));
+        int chunks = 0;
+        for (int i = 0; i < a.n_arrays; i++) {
+            a.arrays[i] = arrays[first + i];
+            a.arrays[i].first_chunk = chunks;
+            chunks += (a.arrays[i].page_bytes + kCopyChunk - 1) / kCopyChunk;
+        }
+        for (int p0 = 0; p0 < n; p0 += kPairs) {
+            const int m = std::min(kPairs, n - p0);
+            for (int i = 0; i < m; i++) a.pairs[i] = make_int2(src[p0 + i], dst[p0 + i]);
+            copy_pages_kernel<kArrays, kPairs><<<dim3(chunks, m), 256, 0, st>>>(a);
+            PAGED_CUDA(cudaGetLastError());
+        }
+    }
+    return FP4ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp4attn_rotary_table(const double* freqs, int pairs, int64_t max_positions, double factor, float* table, void* stream)
+{
+    host::clear_error();
+    if (!freqs || !table || !aligned(table, 16)) return fail(FP4ATTN_EINVAL, "null or misaligned pointer");
+    if (pairs < 1 || pairs > 128 || max_positions < 1) return fail(FP4ATTN_EINVAL, "pairs in [1, 128], max_positions >= 1");
+    for (int i = 0; i < pairs; i++)
+        if (!std::isfinite(freqs[i])) return fail(FP4ATTN_EINVAL, "freqs[%d] is not finite", i);
+    if (!std::isfinite(factor)) return fail(FP4ATTN_EINVAL, "factor is not finite");
+    if (int rc = host::ready()) return rc;
+    RotaryFreqs f{};
+    std::memcpy(f.f, freqs, pairs * sizeof(double));
+    const int64_t blocks = std::min<int64_t>((max_positions * pairs + 255) / 256, 148 * 32);
+    rotary_table_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        f, pairs, max_positions, factor, reinterpret_cast<float2*>(table));
+    PAGED_CUDA(cudaGetLastError());
+    return FP4ATTN_OK;
+}
+
+int fp4attn_rotary(const void* x, void* y, int dtype, int batch, int heads, int seq, int head_dim,
+                   const int64_t* x_strides, const int64_t* y_strides, const float* table, int rotary_dim,
+                   int64_t max_positions, const int32_t* positions, int64_t positions_stride, int interleaved, int inverse,
+                   void* stream)
+{
+    host::clear_error();
+    if (bad_dtype(dtype)) return fail(FP4ATTN_EINVAL, "dtype %d", dtype);
+    if (batch < 0 || heads < 0 || seq < 0 || batch > 65535 || heads > 65535)
+        return fail(FP4ATTN_EINVAL, "batch and heads in [0, 65535], seq >= 0");
+    if (!supported_dim(head_dim))
+        return fail(FP4ATTN_EUNSUPPORTED, "head_dim %d is not one of 32/64/96/128/160/256", head_dim);
+    if (int rc = check_rotary(table, rotary_dim, max_positions, head_dim)) return rc;
+    if (!positions && seq > max_positions) return fail(FP4ATTN_EINVAL, "seq %d exceeds the table's %lld positions", seq,
+                                                       static_cast<long long>(max_positions));
+    if (batch == 0 || heads == 0 || seq == 0) return FP4ATTN_OK;
+    if (!x || !y || !x_strides || !y_strides) return fail(FP4ATTN_EINVAL, "null pointer");
+    if (!aligned(x, bytes_of(dtype)) || !aligned(y, bytes_of(dtype)) || !aligned(positions, 4))
+        return fail(FP4ATTN_EINVAL, "misaligned pointer");
+    if (int rc = host::ready()) return rc;
+    RotaryArgs a{x, y, x_strides[0], x_strides[1], x_strides[2], y_strides[0], y_strides[1], y_strides[2],
+                 heads, seq, head_dim, rotary_dim, reinterpret_cast<const float2*>(table), positions, positions_stride,
+                 max_positions, inverse ? -1.f : 1.f, 1};
+    const bool vec = whole_eights(rotary_dim, interleaved) && wide(x, dtype, {a.xb, a.xh, a.xs}) &&
+                     wide(y, dtype, {a.yb, a.yh, a.ys});
+    const int64_t turned = vec ? (interleaved ? rotary_dim / 8 : rotary_dim / 16) : rotary_dim / 2;
+    const int64_t work = seq * (turned + (head_dim - rotary_dim) / (vec ? 8 : 1));
+    if (work > 0x7FFFFF00) return fail(FP4ATTN_EINVAL, "seq %d is too long", seq);
+    while (a.heads_per_thread < 8 && work * batch * (heads / (2 * a.heads_per_thread)) >= 148 * 2048) a.heads_per_thread *= 2;
+    const dim3 grid(static_cast<unsigned>((work + 255) / 256), (heads + a.heads_per_thread - 1) / a.heads_per_thread, batch);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FP4ATTN_F16) launch_rotary<__half>(grid, st, a, vec, interleaved != 0);
+    else launch_rotary<float>(grid, st, a, vec, interleaved != 0);
+    PAGED_CUDA(cudaGetLastError());
+    return FP4ATTN_OK;
+}
+
+int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* V, const void* Q, void* Q_out, int dtype,
+                         int tokens, int q_heads, const int64_t* k_strides, const int64_t* v_strides,
+                         const int64_t* q_strides, const int32_t* block_table, int64_t table_stride, int seqs,
+                         int max_pages, const int32_t* seq_ids, const int32_t* positions, const float* table,
+                         int rotary_dim, int64_t max_positions, int interleaved, int scale_mode, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_cache(cache)) return rc;
+    if (bad_dtype(dtype)) return fail(FP4ATTN_EINVAL, "dtype %d", dtype);
+    if (scale_mode != FP4ATTN_SCALE_REFERENCE && scale_mode != FP4ATTN_SCALE_OCP)
+        return fail(FP4ATTN_EINVAL, "scale_mode %d", scale_mode);
+    if (tokens < 0) return fail(FP4ATTN_EINVAL, "tokens must be >= 0");
+    if (int rc = check_table(block_table, table_stride, seqs, max_pages)) return rc;
+    if (!seq_ids && tokens != seqs) return fail(FP4ATTN_EINVAL, "without seq_ids there is one token per sequence");
+    if (table)
+        if (int rc = check_rotary(table, rotary_dim, max_positions, cache->head_dim)) return rc;
+    if (!Q != !Q_out || (Q && (q_heads < 1 || q_heads > 65535))) return fail(FP4ATTN_EINVAL, "Q and Q_out go together, with q_heads in [1, 65535]");
+    if (tokens == 0) return FP4ATTN_OK;
+    if (!K || !V || !positions || !k_strides || !v_strides || (Q && !q_strides)) return fail(FP4ATTN_EINVAL, "null pointer");
+    const int es = bytes_of(dtype);
+    if (!aligned(K, es) || !aligned(V, es) || !aligned(Q, es) || !aligned(Q_out, 16) || !aligned(positions, 4) ||
+        !aligned(seq_ids, 4) || !aligned(block_table, 4))
+        return fail(FP4ATTN_EINVAL, "misaligned pointer");
+    if (int rc = host::ready()) return rc;
+    AppendArgs a{};
+    a.k = K; a.v = V; a.q = Q; a.q_out = Q_out;
+    a.kt = k_strides[0]; a.kh = k_strides[1];
+    a.vt = v_strides[0]; a.vh = v_strides[1];
+    if (Q) { a.qt = q_strides[0]; a.qh = q_strides[1]; }
+    a.tokens = tokens;
+    a.q_heads = Q ? q_heads : 0;
+    a.c = view_of(*cache);
+    a.t = TableView{block_table, table_stride, seqs, max_pages};
+    a.seq_ids = seq_ids;
+    a.positions = positions;
+    a.table = reinterpret_cast<const float2*>(table);
+    a.rot = table ? rotary_dim : 0;
+    a.max_positions = max_positions;
+    a.interleaved = interleaved != 0;
+    a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
+    a.vec = whole_eights(a.rot, a.interleaved) && wide(K, dtype, {a.kt, a.kh}) && wide(V, dtype, {a.vt, a.vh}) &&
+            (!Q || wide(Q, dtype, {a.qt, a.qh}));
+    const int64_t units = static_cast<int64_t>(tokens) * (2 * a.c.kv_heads + a.q_heads) * (a.c.head_dim / 8);
+    if ((units + 255) / 256 > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "%d tokens are too many", tokens);
+    const unsigned grid = static_cast<unsigned>((units + 255) / 256);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FP4ATTN_F16) cache_append_kernel<__half><<<grid, 256, 0, st>>>(a);
+    else cache_append_kernel<float><<<grid, 256, 0, st>>>(a);
+    PAGED_CUDA(cudaGetLastError());
+    return FP4ATTN_OK;
+}
+
+int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table, int64_t table_stride, int seqs,
+                         int max_pages, const int32_t* starts, const int32_t* lengths, int max_length, int heads, void* K,
+                         void* V, int dtype, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_cache(cache)) return rc;
+    if (bad_dtype(dtype)) return fail(FP4ATTN_EINVAL, "dtype %d", dtype);
+    if (int rc = check_table(block_table, table_stride, seqs, max_pages)) return rc;
+    if (heads < 1 || heads % cache->kv_heads) return fail(FP4ATTN_EINVAL, "heads %d is not a multiple of kv_heads %d", heads, cache->kv_heads);
+    if (max_length < 0 || seqs > 65535) return fail(FP4ATTN_EINVAL, "max_length >= 0, at most 65535 sequences");
+    if (seqs == 0 || max_length == 0) return FP4ATTN_OK;
+    if (!lengths || !K || !V || !aligned(K, 16) || !aligned(V, 16) || !aligned(lengths, 4) || !aligned(starts, 4) ||
+        !aligned(block_table, 4))
+        return fail(FP4ATTN_EINVAL, "null or misaligned pointer");
+    if (int rc = host::ready()) return rc;
+    const GatherArgs a{view_of(*cache), TableView{block_table, table_stride, seqs, max_pages}, starts, lengths,
+                       max_length, heads / cache->kv_heads, K, V};
+    const int64_t units = static_cast<int64_t>(max_length) * (cache->head_dim / 8);
+    const dim3 grid(static_cast<unsigned>((units + 255) / 256), cache->kv_heads, seqs);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FP4ATTN_F16) cache_gather_kernel<__half><<<grid, 256, 0, st>>>(a);
+    else cache_gather_kernel<float><<<grid, 256, 0, st>>>(a);
+    PAGED_CUDA(cudaGetLastError());
+    return FP4ATTN_OK;
+}
+
+size_t fp4attn_paged_attention_workspace_size(int batch, int q_heads, int kv_heads, int head_dim)
+{
+    if (batch < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || !supported_dim(head_dim)) return 0;
+    return 256;
+}
+
+int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out, float* lse, int in_dtype, int out_dtype,
+                            int batch, int q_heads, const int64_t* q_strides, const int32_t* block_table,
+                            int64_t table_stride, int max_pages, const int32_t* seq_lens, float softmax_scale,
+                            int scale_mode, void* workspace, size_t workspace_bytes, void* stream)
+{
+    host::clear_error();
+    if (int rc = check_cache(cache)) return rc;
+    if (bad_dtype(in_dtype) || bad_dtype(out_dtype)) return fail(FP4ATTN_EINVAL, "dtype %d, %d", in_dtype, out_dtype);
+    if (scale_mode != FP4ATTN_SCALE_REFERENCE && scale_mode != FP4ATTN_SCALE_OCP)
+        return fail(FP4ATTN_EINVAL, "scale_mode %d", scale_mode);
+    if (batch < 0 || batch > 65535) return fail(FP4ATTN_EINVAL, "batch %d in [0, 65535]", batch);
+    if (q_heads < 1 || q_heads % cache->kv_heads)
+        return fail(FP4ATTN_EINVAL, "q_heads %d is not a multiple of kv_heads %d", q_heads, cache->kv_heads);
+    if (int rc = check_table(block_table, table_stride, batch, max_pages)) return rc;
+    if (batch == 0) return FP4ATTN_OK;
+    if (!Q || !Out || !q_strides || !seq_lens) return fail(FP4ATTN_EINVAL, "null pointer");
+    if (!wide(Q, in_dtype, {q_strides[0], q_strides[1]}) || !aligned(Out, 16) || !aligned(lse, 4) || !aligned(seq_lens, 4) ||
+        !aligned(block_table, 4))
+        return fail(FP4ATTN_EINVAL, "Q (and its strides) and Out must be 16-byte aligned");
+    const size_t need = fp4attn_paged_attention_workspace_size(batch, q_heads, cache->kv_heads, cache->head_dim);
+    if (!workspace || workspace_bytes < need)
+        return fail(FP4ATTN_EWORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
+    if (!aligned(workspace, 256)) return fail(FP4ATTN_EINVAL, "workspace must be 256-byte aligned");
+    if (int rc = host::ready()) return rc;
+    PagedArgs a{};
+    a.q = Q;
+    a.qb = q_strides[0];
+    a.qh = q_strides[1];
+    a.batch = batch;
+    a.q_heads = q_heads;
+    a.group = q_heads / cache->kv_heads;
+    a.c = view_of(*cache);
+    a.t = TableView{block_table, table_stride, batch, max_pages};
+    a.seq_lens = seq_lens;
+    const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(cache->head_dim));
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
+    a.out = Out;
+    a.lse = lse;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (in_dtype == FP4ATTN_F16)
+        return out_dtype == FP4ATTN_F16 ? launch_attention<__half, __half>(a, st) : launch_attention<__half, float>(a, st);
+    return out_dtype == FP4ATTN_F16 ? launch_attention<float, __half>(a, st) : launch_attention<float, float>(a, st);
+}
+
+int fp4attn_copy_pages(const fp4attn_cache* caches, int n_caches, const int32_t* src, const int32_t* dst, int n, void* stream)
+{
+    host::clear_error();
+    if (n_caches < 0 || n < 0 || (n_caches && !caches) || (n && (!src || !dst))) return fail(FP4ATTN_EINVAL, "null pointer or negative count");
+    try {
+        std::vector<CopyArray> arrays;
+        int pages = 0x7FFFFFFF;
+        for (int i = 0; i < n_caches; i++) {
+            const fp4attn_cache& c = caches[i];
+            if (int rc = check_cache(&c)) return rc;
+            const int rows = c.kv_heads * c.page_size;
+            arrays.push_back({static_cast<uint8_t*>(c.v), c.v_stride, rows * c.head_dim * 2, 0});
+            arrays.push_back({c.k_codes, c.k_codes_stride, rows * c.head_dim / 2, 0});
+            arrays.push_back({c.k_scales, c.k_scales_stride, rows * c.head_dim / 32, 0});
+            pages = std::min(pages, c.pages);
+        }
+        // Every copy reads what was there before the call: no page is written
+        // twice, and none is both read and written.
+        if (n_caches && n) {
+            std::vector<uint8_t> seen(pages, 0);
+            for (int i = 0; i < n; i++) {
+                if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
+                    return fail(FP4ATTN_EINVAL, "pair %d (%d to %d): page outside [0, %d)", i, src[i], dst[i], pages);
+                if (seen[dst[i]]) return fail(FP4ATTN_EINVAL, "page %d is written twice", dst[i]);
+                seen[dst[i]] = 1;
+            }
+            for (int i = 0; i < n; i++)
+                if (seen[src[i]]) return fail(FP4ATTN_EINVAL, "page %d is both read and written", src[i]);
+        }
+        if (n_caches == 0 || n == 0) return FP4ATTN_OK;
+        if (int rc = host::ready()) return rc;
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (arrays.size() <= 24 && n <= 64) return launch_copies<24, 64>(arrays, src, dst, n, st);
+        return launch_copies<192, 2048>(arrays, src, dst, n, st);
+    } catch (const std::bad_alloc&) {
+        return fail(FP4ATTN_EINVAL, "out of host memory");
+    }
+}
+
+}  // extern "C"

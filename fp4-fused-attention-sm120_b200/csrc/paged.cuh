@@ -1,0 +1,328 @@
+// paged.cuh -- the paged FP4 key / FP16 value cache (sm_100a): appending
+// tokens (keys rotated and quantised on the way in), reading tokens back, and
+// copying pages.
+//
+// One cache holds, per page and key/value head, page_size tokens:
+//   k_codes  [pages][kv_heads][page_size][head_dim / 2]   two E2M1 codes a byte
+//   k_scales [pages][kv_heads][page_size][head_dim / 32]  UE8M0 bytes
+//   v        [pages][kv_heads][page_size][head_dim]       FP16
+// in the row-major forms of fp4attn_quantize, except that a scale of 255
+// (only ever with all-zero codes) is stored as 254, which the tensor core
+// reads as a finite factor.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "device_status.cuh"
+#include "quantize.cuh"
+#include "rotary.cuh"
+
+namespace fp4attn {
+
+struct CacheView {
+    uint8_t* k_codes;
+    uint8_t* k_scales;
+    __half* v;
+    int64_t k_codes_stride, k_scales_stride, v_stride;  // bytes from one page to the next
+    int pages, page_size, page_shift, kv_heads, head_dim;
+};
+
+struct TableView {
+    const int32_t* pages;  // [seqs][stride]
+    int64_t stride;
+    int seqs, max_pages;
+};
+
+// The page of a sequence's position, or -1 (recorded) when there is none.
+__device__ __forceinline__ int page_of(const CacheView& c, const TableView& t, int seq, int pos)
+{
+    if (seq < 0 || seq >= t.seqs) {
+        record_index_error(kIndexSequence, seq);
+        return -1;
+    }
+    const int slot = pos >> c.page_shift;
+    if (slot >= t.max_pages) {
+        record_index_error(kIndexLength, pos);
+        return -1;
+    }
+    const int page = t.pages[seq * t.stride + slot];
+    if (page < 0 || page >= c.pages) {
+        record_index_error(kIndexPage, page);
+        return -1;
+    }
+    return page;
+}
+
+// Eight elements of a block of 32 whose scale byte is sb, encoded as
+// encode32 of quantize.cuh does (see there for the ties).
+template <typename T>
+__device__ __forceinline__ uint32_t encode8(const float (&v)[8], uint32_t sb)
+{
+    const int s = static_cast<int>(sb) - 127;
+    if (s == 128) return 0u;
+    const float inv = exact_pow2_neg(s);
+    float q[8];
+    bool exact = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        q[i] = v[i] * inv;
+        if constexpr (sizeof(T) == 2) {
+            exact |= isnan(v[i]);
+        } else {
+            const uint32_t b = __float_as_uint(q[i]);
+            exact |= ((b << 11) == 0u && b != 0u) || isnan(q[i]);
+        }
+    }
+    if (exact) {
+        uint32_t w = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w |= encode_e2m1(q[i]) << (4 * i);
+        return w;
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[i] = __fmaf_rn(q[i], 1.0f + 0x1p-12f, 0.f);
+    }
+    return ptx::cvt_e2m1x8(q);
+}
+
+struct AppendArgs {
+    const void *k, *v, *q;
+    void* q_out;                       // [tokens][q_heads][head_dim], contiguous
+    int64_t kt, kh, vt, vh, qt, qh;    // element strides of token and head
+    int tokens, q_heads;
+    CacheView c;
+    TableView t;
+    const int32_t* seq_ids;            // [tokens] or null: token i belongs to sequence i
+    const int32_t* positions;          // [tokens]; negative: the token is padding
+    const float2* table;               // rotary table or null
+    int rot;
+    int64_t max_positions;
+    int interleaved, ocp;
+    int vec;                           // 16-byte loads and whole eights in the rotary layout
+};
+
+// Eight elements e0 .. e0 + 7 of a row, rotated (FP32, not yet rounded).
+template <typename T>
+__device__ __forceinline__ void rotated8(const T* row, int e0, const float2* cs, int rot, int interleaved, int vec,
+                                         float (&v)[8])
+{
+    const int half = rot / 2;
+    if (vec) {
+        load8v(row + e0, v);
+        if (e0 >= rot) return;
+        if (interleaved) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 f = __ldg(cs + e0 / 2 + i);
+                turn(v[2 * i], v[2 * i + 1], f.x, f.y, v[2 * i], v[2 * i + 1]);
+            }
+        } else {
+            const bool first = e0 < half;
+            float w[8];
+            load8v(row + (first ? e0 + half : e0 - half), w);
+            const float2* f8 = cs + (first ? e0 : e0 - half);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(f8 + i));
+                float ra, rb;
+                turn(first ? v[i] : w[i], first ? w[i] : v[i], f.x, f.y, ra, rb);
+                v[i] = first ? ra : rb;
+                turn(first ? v[i + 1] : w[i + 1], first ? w[i + 1] : v[i + 1], f.z, f.w, ra, rb);
+                v[i + 1] = first ? ra : rb;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int e = e0 + i;
+        if (e >= rot) {
+            v[i] = to_float(row[e]);
+            continue;
+        }
+        const int j = interleaved ? e / 2 : (e < half ? e : e - half);
+        const int ia = interleaved ? 2 * j : j, ib = interleaved ? 2 * j + 1 : j + half;
+        float ra, rb;
+        turn(to_float(row[ia]), to_float(row[ib]), cs[j].x, cs[j].y, ra, rb);
+        v[i] = e == ia ? ra : rb;
+    }
+}
+
+// One thread per eight elements of a token's K, V or Q; four neighbouring
+// lanes share a block of 32 and its scale.
+template <typename T>
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a)
+{
+    const int D = a.c.head_dim, row8 = D / 8;
+    const int kv_units = a.c.kv_heads * row8, units = 2 * kv_units + (a.q ? a.q_heads * row8 : 0);
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (n >= static_cast<int64_t>(a.tokens) * units) return;
+    const int tok = static_cast<int>(n / units);
+    int u = static_cast<int>(n % units);
+    const int pos = a.positions[tok];
+    const bool is_q = u >= 2 * kv_units;
+    const bool is_v = !is_q && u >= kv_units;
+    u -= is_q ? 2 * kv_units : is_v ? kv_units : 0;
+    const int head = u / row8, e0 = (u % row8) * 8;
+    if (pos < 0) {  // padding: nothing enters the cache, the query row is zero
+        if (is_q) {
+            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            store8v(static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + head) * D + e0, z);
+        }
+        return;
+    }
+    const bool angle_ok = !a.table || pos < a.max_positions;
+    if (!angle_ok) record_index_error(kIndexPosition, pos);
+    const float2* cs = a.table ? a.table + (angle_ok ? pos : 0) * static_cast<int64_t>(a.rot / 2) : nullptr;
+    float v[8];
+    if (is_q) {
+        if (!angle_ok) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 0.f;
+        } else
+            rotated8(static_cast<const T*>(a.q) + tok * a.qt + head * a.qh, e0, cs, a.rot, a.interleaved, a.vec, v);
+        store8v(static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + head) * D + e0, v);
+        return;
+    }
+    const int page = page_of(a.c, a.t, a.seq_ids ? a.seq_ids[tok] : tok, pos);
+    if (page < 0 || !angle_ok) return;
+    const int64_t in_page = static_cast<int64_t>(head) * a.c.page_size + (pos & (a.c.page_size - 1));
+    if (is_v) {
+        const T* row = static_cast<const T*>(a.v) + tok * a.vt + head * a.vh + e0;
+        __half* dst = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.c.v) + page * a.c.v_stride) + in_page * D + e0;
+        if constexpr (sizeof(T) == 2) {  // FP16 values keep their bits
+            if (a.vec) {
+                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(row);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) dst[i] = row[i];
+            }
+        } else {
+            if (a.vec) {
+                load8v(row, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = row[i];
+            }
+            store8v(dst, v);
+        }
+        return;
+    }
+    rotated8(static_cast<const T*>(a.k) + tok * a.kt + head * a.kh, e0, cs, a.rot, a.interleaved, a.vec, v);
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        v[i] = to_float(from_float<T>(v[i]));  // the key as a separate rotation would have left it
+        amax = fmaxf(amax, fabsf(v[i]));
+    }
+    const uint32_t quad = 0xFu << ((threadIdx.x & 31) & ~3);
+    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+    const uint32_t sb = scale_byte(amax, a.ocp);
+    const uint32_t w = encode8<T>(v, sb);
+    *reinterpret_cast<uint32_t*>(a.c.k_codes + page * a.c.k_codes_stride + in_page * (D / 2) + e0 / 2) = w;
+    if ((u & 3) == 0)
+        a.c.k_scales[page * a.c.k_scales_stride + in_page * (D / 32) + e0 / 32] =
+            static_cast<uint8_t>(sb == 255u ? 254u : sb);
+}
+
+// Exactly 2^(sb - 127).
+__device__ __forceinline__ float scale_value(uint32_t sb)
+{
+    return sb ? __uint_as_float(sb << 23) : __uint_as_float(1u << 22);
+}
+
+// The value of E2M1 code n (sign in bit 3), unscaled.
+__device__ __forceinline__ float e2m1_value(uint32_t n)
+{
+    // Twice the magnitudes 0, 1, 2, 3, 4, 6, 8, 12 of bits 0-2, a nibble each.
+    const float m = static_cast<float>((0xC8643210u >> (4u * (n & 7u))) & 15u) * 0.5f;
+    return n & 8u ? -m : m;
+}
+
+struct GatherArgs {
+    CacheView c;
+    TableView t;
+    const int32_t *starts, *lengths;  // [seqs]; starts may be null (0)
+    int max_length, repeat;           // every key/value head is written `repeat` times
+    void *k, *v;                      // [seqs][kv_heads * repeat][max_length][head_dim]
+};
+
+// One thread per eight elements of a token's K and V of one head; rows past a
+// sequence's length are written as zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) cache_gather_kernel(const GatherArgs a)
+{
+    const int D = a.c.head_dim, row8 = D / 8;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (n >= static_cast<int64_t>(a.max_length) * row8) return;
+    const int head = blockIdx.y, seq = blockIdx.z;
+    const int i = static_cast<int>(n / row8), e0 = static_cast<int>(n % row8) * 8;
+    float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const int start = a.starts ? a.starts[seq] : 0, length = a.lengths[seq];
+    if (start < 0 || length < 0 || length > a.max_length) {
+        if (n == 0 && head == 0) record_index_error(kIndexLength, start < 0 ? start : length);
+    } else if (i < length) {
+        const int64_t pos = static_cast<int64_t>(start) + i;
+        const int page = pos > 0x7FFFFFFF ? -1 : page_of(a.c, a.t, seq, static_cast<int>(pos));
+        if (page >= 0) {
+            const int64_t in_page = static_cast<int64_t>(head) * a.c.page_size + (pos & (a.c.page_size - 1));
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(a.c.k_codes + page * a.c.k_codes_stride +
+                                                                  in_page * (D / 2) + e0 / 2);
+            const float sc = scale_value(a.c.k_scales[page * a.c.k_scales_stride + in_page * (D / 32) + e0 / 32]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) k[j] = e2m1_value((w >> (4 * j)) & 15u) * sc;
+            load8v(reinterpret_cast<const __half*>(reinterpret_cast<const uint8_t*>(a.c.v) + page * a.c.v_stride) +
+                       in_page * D + e0, v);
+        }
+    }
+    for (int r = 0; r < a.repeat; r++) {
+        const int64_t at = ((static_cast<int64_t>(seq) * a.c.kv_heads + head) * a.repeat + r) * a.max_length + i;
+        store8v(static_cast<T*>(a.k) + at * D + e0, k);
+        store8v(static_cast<T*>(a.v) + at * D + e0, v);
+    }
+}
+
+// ---------------------------------------------------------------- page copies
+constexpr int kCopyChunk = 16384;  // bytes a block copies: 256 threads, four 16-byte words each
+
+struct CopyArray {
+    uint8_t* base;
+    int64_t page_stride;
+    int page_bytes;
+    int first_chunk;  // chunks of the arrays before this one
+};
+
+// The arrays and page pairs of one launch, by value: the pairs are the host's
+// and are checked there, and a captured launch carries them with it.
+template <int kArrays, int kPairs>
+struct CopyArgs {
+    CopyArray arrays[kArrays];
+    int2 pairs[kPairs];  // source, destination
+    int n_arrays;
+};
+
+// Block (x, y): chunk x of pair y.
+template <int kArrays, int kPairs>
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyArgs<kArrays, kPairs> a)
+{
+    int i = 0;
+    while (i + 1 < a.n_arrays && a.arrays[i + 1].first_chunk <= static_cast<int>(blockIdx.x)) i++;
+    const CopyArray& ar = a.arrays[i];
+    const int2 p = a.pairs[blockIdx.y];
+    const uint4* src = reinterpret_cast<const uint4*>(ar.base + p.x * ar.page_stride);
+    uint4* dst = reinterpret_cast<uint4*>(ar.base + p.y * ar.page_stride);
+    const int words = ar.page_bytes / 16;
+    const int w0 = (static_cast<int>(blockIdx.x) - ar.first_chunk) * (kCopyChunk / 16) + threadIdx.x;
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (w0 + 256 * j < words) v[j] = src[w0 + 256 * j];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (w0 + 256 * j < words) dst[w0 + 256 * j] = v[j];
+}
+
+}  // namespace fp4attn

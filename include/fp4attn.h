@@ -48,7 +48,10 @@ typedef enum {
     FP4ATTN_ECUDA = 3,        /* a CUDA runtime or driver call failed          */
     FP4ATTN_ETIMEOUT = 4,     /* a kernel's bounded wait expired (reported by  */
                               /* fp4attn_status_query after the stream syncs) */
-    FP4ATTN_EWORKSPACE = 5    /* workspace missing or too small               */
+    FP4ATTN_EWORKSPACE = 5,   /* workspace missing or too small               */
+    FP4ATTN_EINDEX = 6        /* a position, page, sequence or length that a  */
+                              /* kernel read was out of range (reported by    */
+                              /* fp4attn_status_query after the stream syncs) */
 } fp4attn_status;
 
 /* ---- element types ------------------------------------------------------ */
@@ -247,8 +250,8 @@ int fp4attn_debug_scores(const void* Q, const void* K, float* S, int in_dtype, i
                          size_t workspace_bytes, void* stream);
 
 /* Reads and clears the device error word that kernels set when a bounded
- * wait expires.  Synchronises `stream` first.  Returns FP4ATTN_OK or
- * FP4ATTN_ETIMEOUT (or FP4ATTN_ECUDA if the query itself fails).  The word is
+ * wait expires or an index is out of range.  Synchronises `stream` first.
+ * Returns FP4ATTN_OK, FP4ATTN_ETIMEOUT or FP4ATTN_EINDEX (or FP4ATTN_ECUDA if the query itself fails).  The word is
  * one per device, shared by every stream: a kernel still running on another
  * stream may set it after this call returns (it is then reported by the next
  * query), and a timeout raised on another stream is reported by whichever
@@ -279,6 +282,105 @@ int fp4attn_selftest_abort(const void* V, void* Out, int batch, int heads, int s
  * uses for part of its exponentials (n even, 16-byte aligned device arrays).
  * No counterpart in the reference, whose softmax calls expf (common.h:236). */
 int fp4attn_selftest_exp2(const float* x, float* y, int64_t n, void* stream);
+
+/* ---- serving: rotary positions, the paged cache, attention over it --------
+ * The reference has none of these (it attends over whole K and V tensors,
+ * common.h:68-77).  All are asynchronous on `stream`, keep nothing between
+ * calls and may be captured into CUDA graphs.  Positions, pages, sequence
+ * numbers and lengths that a kernel reads from device memory are checked
+ * there: what is out of range is not accessed, and the next
+ * fp4attn_status_query reports FP4ATTN_EINDEX. */
+
+/* table[p][j] = factor * (cos, sin)(p * freqs[j]) as FP32, [max_positions]
+ * [pairs][2], the angles in 64 bits.  freqs: `pairs` doubles (1 to 128) in
+ * host memory.  Long-context scalings change freqs and factor. */
+int fp4attn_rotary_table(const double* freqs, int pairs, int64_t max_positions, double factor, float* table,
+                         void* stream);
+
+/* Rotary positions: y = x with the first rotary_dim (even) elements of every
+ * row turned pair by pair by the angles of the row's position, the rest
+ * copied.  Pairs are (2j, 2j+1) when `interleaved`, else (j, j+rotary_dim/2).
+ * x, y: [batch, heads, seq, head_dim] with element strides {batch, head, seq}
+ * (the last dimension contiguous), F16 or F32; y may be x itself (with the
+ * same strides).  positions: [batch][seq] with positions_stride elements from
+ * one batch entry to the next (0: shared), or null for 0 .. seq-1; a position
+ * outside [0, max_positions) gives a row of zeros and FP4ATTN_EINDEX.
+ * inverse: turned back by the same angles (the transpose), which is the
+ * gradient: dx = fp4attn_rotary(dy, inverse).  Products and sums are rounded
+ * to FP32 one by one and the result once to the tensor's type. */
+int fp4attn_rotary(const void* x, void* y, int dtype, int batch, int heads, int seq, int head_dim,
+                   const int64_t* x_strides, const int64_t* y_strides, const float* table, int rotary_dim,
+                   int64_t max_positions, const int32_t* positions, int64_t positions_stride, int interleaved,
+                   int inverse, void* stream);
+
+/* One layer's paged cache: keys as E2M1 codes with UE8M0 scales (the
+ * row-major forms of fp4attn_quantize, but with 255 stored as 254), values as
+ * FP16.  Within a page everything is contiguous; the strides (bytes from one
+ * page to the next, multiples of 16) let a page hold several layers.
+ * page_size: 16, 32, 64 or 128 tokens; pointers 16-byte aligned. */
+typedef struct {
+    uint8_t* k_codes;  /* [pages][kv_heads][page_size][head_dim / 2]  */
+    uint8_t* k_scales; /* [pages][kv_heads][page_size][head_dim / 32] */
+    void* v;           /* [pages][kv_heads][page_size][head_dim] FP16 */
+    int64_t k_codes_stride, k_scales_stride, v_stride;
+    int pages, page_size, kv_heads, head_dim;
+} fp4attn_cache;
+
+/* Puts new tokens into a cache: each key is rotated (when `table` is given),
+ * rounded to its type and quantised by scale_mode; each value is rounded to
+ * FP16; and, when Q is given, each query is rotated into Q_out.  K, V:
+ * [tokens, kv_heads, head_dim], Q: [tokens, q_heads, head_dim], with element
+ * strides {token, head}; Q_out: the same, contiguous.
+ * Token i is token positions[i] of sequence seq_ids[i] (null: sequence i), and
+ * lies in page block_table[seq * table_stride + position / page_size].  A
+ * negative position marks padding: it leaves the cache alone and gives a zero
+ * query row; so does a position beyond the rotary table, as FP4ATTN_EINDEX.
+ * The codes and scales are byte for byte those of fp4attn_rotary followed by
+ * fp4attn_quantize.  No two tokens of a call may have the same place in the
+ * cache. */
+int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* V, const void* Q, void* Q_out,
+                         int dtype, int tokens, int q_heads, const int64_t* k_strides, const int64_t* v_strides,
+                         const int64_t* q_strides, const int32_t* block_table, int64_t table_stride, int seqs,
+                         int max_pages, const int32_t* seq_ids, const int32_t* positions, const float* table,
+                         int rotary_dim, int64_t max_positions, int interleaved, int scale_mode, void* stream);
+
+/* Reads tokens back: K and V [seqs, heads, max_length, head_dim] of dtype get
+ * the values of tokens starts[s] .. starts[s]+lengths[s]-1 (starts null: 0) of
+ * every sequence, zeros behind them; heads is a multiple of kv_heads, each
+ * key/value head repeated for its query heads.  For attention over a cached
+ * prefix by fp4attn_forward_masked. A key above FP16's range is infinite there. */
+int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table, int64_t table_stride, int seqs,
+                         int max_pages, const int32_t* starts, const int32_t* lengths, int max_length, int heads,
+                         void* K, void* V, int dtype, void* stream);
+
+/* Workspace bytes of fp4attn_paged_attention (0 for an invalid shape); it does
+ * not depend on the lengths. */
+size_t fp4attn_paged_attention_workspace_size(int batch, int q_heads, int kv_heads, int head_dim);
+
+/* Attention of one new token per sequence over the cache: Out[b][h] =
+ * softmax(softmax_scale * Qq Kq^T) V over the first seq_lens[b] tokens of
+ * sequence b (its own included, once appended), what fp4attn_forward gives for
+ * that one query row.  Q: [batch, q_heads, head_dim] of in_dtype with element
+ * strides {batch, head}; query head h reads key/value head
+ * h / (q_heads / kv_heads).  Out: [batch, q_heads, head_dim] of out_dtype,
+ * lse (or null): [batch, q_heads] natural log-sum-exp.  A sequence of length
+ * 0 gives zeros and +inf.  Several new tokens of one sequence are as many
+ * rows that share its pages, with lengths that grow by one.
+ * softmax_scale <= 0 selects 1/sqrt(head_dim).  workspace: as
+ * fp4attn_paged_attention_workspace_size says, 256-byte aligned, any content;
+ * not shared with another call in flight. */
+int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out, float* lse, int in_dtype,
+                            int out_dtype, int batch, int q_heads, const int64_t* q_strides,
+                            const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
+                            float softmax_scale, int scale_mode, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Copies whole pages, src[i] to dst[i], within each of n_caches caches (the
+ * layers of a model share one page numbering).  src, dst: host memory, read
+ * before the call returns.  A page may be copied to several, but none is
+ * written twice or both read and written (FP4ATTN_EINVAL). */
+int fp4attn_copy_pages(const fp4attn_cache* caches, int n_caches, const int32_t* src, const int32_t* dst, int n,
+                       void* stream);
 
 /* Static description of a status code. */
 const char* fp4attn_error_string(int status);
