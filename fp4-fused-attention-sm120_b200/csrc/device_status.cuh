@@ -30,4 +30,64 @@ __device__ __forceinline__ void record_index_error(int kind, int64_t value)
     }
 }
 
+// Bounded waits, as the attention kernels have them: on expiry the wait records
+// its site, raises the block's abort flag and returns false, and so does every
+// later wait of the block.
+enum ServingSite : int {
+    kPagedKFull = 1,
+    kPagedVFull,
+    kPagedEmpty,
+    kPagedScales,
+    kPagedQFull,
+    kPagedQEmpty,
+    kPagedSFull,
+    kPagedSFree,
+    kPagedPFull,
+    kPagedOFull,
+    kPagedOFree,
+    kPagedDrain,
+};
+
+__device__ __forceinline__ void record_serving_timeout(int site)
+{
+    if (atomicCAS(&g_serving_error[0], 0, 4 /*FP4ATTN_ETIMEOUT*/) == 0) {
+        g_serving_error[1] = site;
+        g_serving_error[2] = blockIdx.x;
+    }
+}
+
+struct ServingWait {
+    volatile int* abort_flag;
+    unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, const ServingWait& w, int site)
+{
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = ptx::globaltimer_ns();
+    for (uint32_t it = 1; it < (1u << 30); ++it) {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if ((it & 31u) == 0u) {
+            if (*w.abort_flag) return false;
+            if (ptx::globaltimer_ns() - t0 > w.timeout_ns) break;
+        }
+    }
+    *w.abort_flag = 1;
+    record_serving_timeout(site);
+    return false;
+}
+
+// On the way out: waits for what is in flight whatever the abort flag says.
+__device__ __forceinline__ void bounded_drain(uint64_t* bar, uint32_t parity, unsigned long long ns)
+{
+    const uint64_t t0 = ptx::globaltimer_ns();
+    for (uint32_t it = 0; it < (1u << 30); ++it) {
+        if (ptx::mbar_try_wait(bar, parity)) return;
+        if ((it & 31u) == 0u && ptx::globaltimer_ns() - t0 > ns) {
+            record_serving_timeout(kPagedDrain);
+            return;
+        }
+    }
+}
+
 }  // namespace fp4attn

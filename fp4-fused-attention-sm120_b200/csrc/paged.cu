@@ -3,12 +3,17 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cudaTypedefs.h>
+
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <mutex>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "../../include/fp4attn.h"
@@ -17,6 +22,7 @@
 #include "rotary.cuh"
 
 namespace fp4attn {
+unsigned long long current_context_id();  // fp4attn.cu
 namespace host {  // fp4attn.cu
 int error(int code, const char* msg);
 void clear_error();
@@ -142,20 +148,125 @@ void launch_rotary(dim3 grid, cudaStream_t st, const RotaryArgs& a, bool vec, bo
     else rotary_kernel<T, false, false><<<grid, 256, 0, st>>>(a);
 }
 
-template <typename InT, typename OutT>
-int launch_attention(const PagedArgs& a, cudaStream_t st)
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
 {
-    const dim3 grid(a.q_heads, a.batch);
-    switch (a.c.head_dim) {
-        case 32: paged_attention_simple_kernel<InT, OutT, 32><<<grid, 128, 0, st>>>(a); break;
-        case 64: paged_attention_simple_kernel<InT, OutT, 64><<<grid, 128, 0, st>>>(a); break;
-        case 96: paged_attention_simple_kernel<InT, OutT, 96><<<grid, 128, 0, st>>>(a); break;
-        case 128: paged_attention_simple_kernel<InT, OutT, 128><<<grid, 128, 0, st>>>(a); break;
-        case 160: paged_attention_simple_kernel<InT, OutT, 160><<<grid, 128, 0, st>>>(a); break;
-        default: paged_attention_simple_kernel<InT, OutT, 256><<<grid, 128, 0, st>>>(a); break;
-    }
-    PAGED_CUDA(cudaGetLastError());
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+int encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+               const cuuint64_t* strides, const cuuint32_t* box, int swizzle_bytes)
+{
+    auto enc = tensor_map_encoder();
+    if (!enc) return fail(FP4ATTN_ECUDA, "cuTensorMapEncodeTiled unavailable");
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+    const CUtensorMapSwizzle sw = swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                  : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                        : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUresult r = enc(m, type, rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FP4ATTN_OK : fail(FP4ATTN_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+}
+
+// Query heads the attention's MMAs take at once, and the groups a key/value
+// head's query heads are split into.
+int mma_heads(int group) { return group <= 16 ? 16 : 32; }
+
+struct AttentionWorkspace {
+    size_t items, ml, o, total;
+};
+
+AttentionWorkspace attention_workspace(int group, int head_dim)
+{
+    const size_t rows = static_cast<size_t>(2 * kPagedBlocks) * mma_heads(group);
+    AttentionWorkspace w{};
+    w.ml = (kPagedBlocks * sizeof(int4) + 255) / 256 * 256;
+    w.o = w.ml + rows * sizeof(float2);
+    w.total = w.o + rows * head_dim * sizeof(float);
+    return w;
+}
+
+template <typename... KArgs, typename... Args>
+int launch_after(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    PAGED_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
     return FP4ATTN_OK;
+}
+
+template <typename OutT, int D, int NH>
+int launch_attention(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
+{
+    using C = PagedCfg<D, NH, sizeof(OutT) == 4>;
+    auto kern = paged_attention_kernel<OutT, D, NH>;
+    // The shared memory limit is an attribute of the kernel in a context.
+    static std::atomic<unsigned long long> done[64];
+    int dev = 0;
+    PAGED_CUDA(cudaGetDevice(&dev));
+    const unsigned long long ctx = current_context_id();
+    if (dev < 0 || dev >= 64) return fail(FP4ATTN_EUNSUPPORTED, "device index %d", dev);
+    if (ctx == 0 || done[dev].load(std::memory_order_acquire) != ctx) {
+        PAGED_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+        done[dev].store(ctx, std::memory_order_release);
+    }
+    const CacheView& c = a.c;
+    CUtensorMap tk, tv;
+    {
+        const cuuint64_t row = D / 2;
+        const cuuint64_t dims[4] = {row, static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.kv_heads),
+                                    static_cast<cuuint64_t>(c.pages)};
+        const cuuint64_t strides[3] = {row, row * c.page_size, static_cast<cuuint64_t>(c.k_codes_stride)};
+        const cuuint32_t box[4] = {C::KROW, static_cast<cuuint32_t>(c.page_size), 1, 1};
+        if (int rc = encode_map(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.k_codes, dims, strides, box, C::KROW)) return rc;
+    }
+    {
+        const cuuint64_t row = D * 2;
+        const cuuint64_t dims[5] = {C::CHE, static_cast<cuuint64_t>(c.page_size), C::DCH,
+                                    static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+        const cuuint64_t strides[4] = {row, C::CB, row * c.page_size, static_cast<cuuint64_t>(c.v_stride)};
+        const cuuint32_t box[5] = {C::CHE, static_cast<cuuint32_t>(c.page_size), C::DCH, 1, 1};
+        if (int rc = encode_map(&tv, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, c.v, dims, strides, box, C::CB)) return rc;
+    }
+    if (int rc = launch_after(kern, dim3(blocks), C::THREADS, C::SMEM_BYTES, st, tk, tv, a)) return rc;
+    if (!join) return FP4ATTN_OK;
+    return launch_after(paged_join_kernel<OutT, D, NH>, dim3(blocks, a.heads_per_group), 128, 0, st, a);
+}
+
+template <typename OutT, int D>
+int launch_heads(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
+{
+    return mma_heads(a.group) == 16 ? launch_attention<OutT, D, 16>(a, blocks, join, st)
+                                    : launch_attention<OutT, D, 32>(a, blocks, join, st);
+}
+
+template <typename OutT>
+int launch_dim(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
+{
+    switch (a.c.head_dim) {
+        case 32: return launch_heads<OutT, 32>(a, blocks, join, st);
+        case 64: return launch_heads<OutT, 64>(a, blocks, join, st);
+        case 96: return launch_heads<OutT, 96>(a, blocks, join, st);
+        case 128: return launch_heads<OutT, 128>(a, blocks, join, st);
+        case 160: return launch_heads<OutT, 160>(a, blocks, join, st);
+        default: return launch_heads<OutT, 256>(a, blocks, join, st);
+    }
 }
 
 template <int kArrays, int kPairs>
@@ -319,7 +430,7 @@ int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table,
 size_t fp4attn_paged_attention_workspace_size(int batch, int q_heads, int kv_heads, int head_dim)
 {
     if (batch < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || !supported_dim(head_dim)) return 0;
-    return 256;
+    return attention_workspace(q_heads / kv_heads, head_dim).total;
 }
 
 int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out, float* lse, int in_dtype, int out_dtype,
@@ -348,6 +459,7 @@ int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out
     if (int rc = host::ready()) return rc;
     PagedArgs a{};
     a.q = Q;
+    a.q_half = in_dtype == FP4ATTN_F16;
     a.qb = q_strides[0];
     a.qh = q_strides[1];
     a.batch = batch;
@@ -361,10 +473,23 @@ int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out
     a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
     a.out = Out;
     a.lse = lse;
+    const int nh = mma_heads(a.group);
+    a.splits = (a.group + nh - 1) / nh;
+    a.heads_per_group = (a.group + a.splits - 1) / a.splits;
+    a.head_groups = cache->kv_heads * a.splits;
+    const AttentionWorkspace ws = attention_workspace(a.group, cache->head_dim);
+    char* base = static_cast<char*>(workspace);
+    a.p = PagedPartials{reinterpret_cast<float*>(base + ws.o), reinterpret_cast<float2*>(base + ws.ml),
+                        reinterpret_cast<int4*>(base + ws.items)};
+    a.timeout_ns = host::timeout_ns();
+    // The most tiles the block table allows; what there are is known on the device.
+    const int64_t longest = (static_cast<int64_t>(max_pages) * cache->page_size + kPagedTile - 1) / kPagedTile;
+    if (longest * a.head_groups > 0x7FFFFFFF / batch)
+        return fail(FP4ATTN_EINVAL, "batch %d x heads x max_pages %d has more than 2^31 tiles", batch, max_pages);
+    const int64_t tiles = longest * a.head_groups * batch;
+    const int blocks = static_cast<int>(std::min<int64_t>({kPagedBlocks, host::sms(), tiles}));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (in_dtype == FP4ATTN_F16)
-        return out_dtype == FP4ATTN_F16 ? launch_attention<__half, __half>(a, st) : launch_attention<__half, float>(a, st);
-    return out_dtype == FP4ATTN_F16 ? launch_attention<float, __half>(a, st) : launch_attention<float, float>(a, st);
+    return out_dtype == FP4ATTN_F16 ? launch_dim<__half>(a, blocks, longest > 1, st) : launch_dim<float>(a, blocks, longest > 1, st);
 }
 
 int fp4attn_copy_pages(const fp4attn_cache* caches, int n_caches, const int32_t* src, const int32_t* dst, int n, void* stream)
