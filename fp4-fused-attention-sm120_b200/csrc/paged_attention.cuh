@@ -26,13 +26,21 @@
 // blocks each writes a partial result (unnormalised O, running maximum, sum),
 // and paged_join_kernel joins them, in order, so results repeat bit for bit.
 //
-// Roles (256 threads):
-//   warp 0     producer: a lane per page of the tile loads its codes, scales
-//              (raw) and values with TMA into a ring of stages.
-//   warp 1     MMA issuer (one thread): S^T of tile g + 1, then O^T of tile g.
-//   warp 2     scales: raw scale bytes to the tensor core's scale layout.
-//   warp 3     queries: quantises the next item's query heads.
-//   warps 4-7  softmax: thread = key (row of S^T), then head-dim row of O^T.
+// Roles (384 threads):
+//   warp 0      key producer: codes by TMA (a lane per page of the tile), raw
+//               scales by cp.async, into a ring of stages.
+//   warp 1      value producer: V by TMA, a lane per page; and the queries:
+//               quantises each item's query heads, some tiles ahead.
+//   warp 2      S^T issuer: brings the scales into the tensor core's layout,
+//               then one thread issues the MMAs.
+//   warp 3      O^T issuer (one thread).
+//   warps 4-11  two softmax warpgroups, which take the items in turn, so that
+//               one starts an item while the other finishes the one before:
+//               thread = key (row of S^T), then head-dim row of O^T.
+// A single thread runs a dependent instruction in about six cycles and passes
+// a ready barrier in about a hundred, and a tile has some 900 (head_dim 64) to
+// 1,800 cycles (128) of the memory's time: one thread that issued both MMAs
+// of a tile took 3,000 (0.196 ms for 64 sequences of up to 8192 tokens).
 //
 // The softmax reference m starts as the item's first tile's maximum and is
 // moved only when a score exceeds it by more than 2^8 (FP16 P would come near
@@ -59,7 +67,7 @@ constexpr int kPagedTile = 128;
 
 template <int D, int NH, bool kSplitP>
 struct PagedCfg {
-    static constexpr int THREADS = 256;
+    static constexpr int THREADS = 384;
     static constexpr int KROW = D <= 64 ? 32 : D <= 128 ? 64 : 128;  // bytes of a key's codes in shared memory (= swizzle)
     static constexpr int KSTEPS = (D + 63) / 64;                     // mxf4 MMAs of K = 64 per S^T tile
     static constexpr int ATOMS = (KSTEPS + 1) / 2;                   // 512-byte scale atoms (four blocks of 32)
@@ -89,10 +97,11 @@ struct PagedCfg {
     static constexpr int STAGE = K_BYTES + V_BYTES + S_BYTES;
     static constexpr int OFF_P = 0;                                  // [2][PARTS][128 keys][PROW]
     static constexpr int P_BYTES = kPagedTile * PROW;
-    static constexpr int OFF_Q = OFF_P + 2 * PARTS * P_BYTES;        // [2][NH rows][KROW]
+    static constexpr int QBUFS = 4;                                  // items whose queries may be ready ahead
+    static constexpr int OFF_Q = OFF_P + 2 * PARTS * P_BYTES;        // [QBUFS][NH rows][KROW]
     static constexpr int Q_BYTES = align1k(NH * KROW);
-    static constexpr int OFF_QSF = OFF_Q + 2 * Q_BYTES;              // [2][ATOMS][512]
-    static constexpr int OFF_KSF = OFF_QSF + 2 * ATOMS * 512;        // [2][ATOMS][512]
+    static constexpr int OFF_QSF = OFF_Q + QBUFS * Q_BYTES;          // [QBUFS][ATOMS][512]
+    static constexpr int OFF_KSF = OFF_QSF + QBUFS * ATOMS * 512;    // [2][ATOMS][512]
     static constexpr int OFF_STAGE = align1k(OFF_KSF + 2 * ATOMS * 512);
     // The O^T MMA reads 128 rows (head-dim columns) of V: past head_dim it
     // reads on into what follows; those rows of O^T are not used.
@@ -110,7 +119,7 @@ struct PagedCfg {
 struct PagedPartials {
     float* o;        // [2 * kPagedBlocks][NH][D]
     float2* ml;      // [2 * kPagedBlocks][NH]  maximum (log2 domain), sum
-    int4* items;     // [kPagedBlocks]  sequence, head group, last block; sequence -1: none begun here spans on
+    int4* items;     // [kPagedBlocks]  sequence, head group, last block, first slot; sequence -1: none begun here goes on
 };
 
 struct PagedArgs {
@@ -148,40 +157,50 @@ __device__ __forceinline__ int paged_first(int64_t total, int block, int blocks)
     return static_cast<int>(total * block / blocks);
 }
 
-// The walk over a block's tiles; every role makes its own.
-struct TileWalk {
-    int b, hg, tile, tiles, len, left;
-    bool first;  // the first tile of an item in this block's range
-    __device__ __forceinline__ void begin(const PagedArgs& a, const int4& start, int n)
+// The walk over the items, or parts of items, in a block's range; every role
+// makes its own.
+struct ItemWalk {
+    int b, hg, tile, n, left;  // the part: its first tile and number of tiles; tiles left in the range, its own included
+    int len, tiles;            // the sequence's
+    __device__ __forceinline__ void begin(const PagedArgs& a, const int4& start, int count)
     {
         b = start.x;
         hg = start.y;
         tile = start.z;
-        left = n;
-        first = true;
+        left = count;
+        n = 0;
         if (left > 0) {
             len = paged_length(a, b);
             tiles = paged_tiles(len);
+            n = min(left, tiles - tile);
         }
     }
-    __device__ __forceinline__ int keys() const { return max(0, min(kPagedTile, len - tile * kPagedTile)); }
-    __device__ __forceinline__ bool last() const { return tile + 1 == tiles || left == 1; }
     __device__ __forceinline__ void next(const PagedArgs& a)
     {
-        left--;
-        tile++;
-        first = false;
-        if (tile == tiles) {
-            tile = 0;
-            first = true;
-            if (++hg == a.head_groups) {
-                hg = 0;
-                b++;
-                if (left > 0) {
-                    len = paged_length(a, b);
-                    tiles = paged_tiles(len);
-                }
-            }
+        left -= n;
+        tile = 0;
+        if (left > 0 && ++hg == a.head_groups) {
+            hg = 0;
+            b++;
+            len = paged_length(a, b);
+            tiles = paged_tiles(len);
+        }
+        n = min(left, tiles);
+    }
+    // Keys of the part's i-th tile.
+    __device__ __forceinline__ int keys(int i) const { return max(0, min(kPagedTile, len - (tile + i) * kPagedTile)); }
+};
+
+// A position in a ring of N stages and the parity of the stage's use.
+template <int N>
+struct Ring {
+    int s = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++s == N) {
+            s = 0;
+            parity ^= 1u;
         }
     }
 };
@@ -194,16 +213,23 @@ struct PagedRange {
     int blocks;        // blocks that have any (the first ones)
 };
 
-// This block's range, by a scan of the lengths with all 256 threads.
+// This block's range, by a scan of the lengths with the first 256 threads
+// (every thread of the block calls it).
 __device__ __forceinline__ void find_range(const PagedArgs& a, PagedRange* range, int* scratch)
 {
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    int sum = 0;
-    for (int b = tid; b < a.batch; b += 256) sum += paged_tiles(paged_length(a, b));
-    for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
-    if (lane == 0) scratch[warp] = sum;
+    const bool scans = tid < 256;
+    int mine = 0, sum = 0;  // tiles of sequence tid; of sequences tid, tid + 256, ...
+    if (scans) {
+        if (tid < a.batch) mine = paged_tiles(paged_length(a, tid));
+        sum = mine;
+        for (int b = tid + 256; b < a.batch; b += 256) sum += paged_tiles(paged_length(a, b));
+        sum = __reduce_add_sync(~0u, sum);
+        if (lane == 0) scratch[warp] = sum;
+    }
     __syncthreads();
     int64_t total = 0;
+#pragma unroll
     for (int i = 0; i < 8; i++) total += scratch[i];
     total *= a.head_groups;
     const int blocks = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
@@ -218,22 +244,24 @@ __device__ __forceinline__ void find_range(const PagedArgs& a, PagedRange* range
     if (idle) return;
     int carry = 0;  // tiles (of one head group) of the sequences before this chunk
     for (int b0 = 0; b0 < a.batch; b0 += 256) {
-        const int mine = b0 + tid < a.batch ? paged_tiles(paged_length(a, b0 + tid)) : 0;
+        if (b0 > 0) mine = scans && b0 + tid < a.batch ? paged_tiles(paged_length(a, b0 + tid)) : 0;
         int inc = mine;
+#pragma unroll
         for (int i = 1; i < 32; i <<= 1) {
             const int v = __shfl_up_sync(~0u, inc, i);
             if (lane >= i) inc += v;
         }
         __syncthreads();
-        if (lane == 31) scratch[warp] = inc;
+        if (scans && lane == 31) scratch[warp] = inc;
         __syncthreads();
         int before = carry, all = 0;
+#pragma unroll
         for (int i = 0; i < 8; i++) {
             if (i < warp) before += scratch[i];
             all += scratch[i];
         }
         const int64_t at = static_cast<int64_t>(before + inc - mine) * a.head_groups;
-        if (t1 > t0 && t0 >= at && t0 < at + static_cast<int64_t>(mine) * a.head_groups) {
+        if (scans && t0 >= at && t0 < at + static_cast<int64_t>(mine) * a.head_groups) {
             const int in = static_cast<int>(t0 - at);
             range->start = make_int4(b0 + tid, in / mine, in % mine, 0);
         }
@@ -241,8 +269,22 @@ __device__ __forceinline__ void find_range(const PagedArgs& a, PagedRange* range
     }
 }
 
+// Of four values per lane: the warp's `op` of the q-th, in the lanes with
+// (lane >> 3) == q.  Six shuffles (each pair of them halves what a lane holds).
+template <typename Op>
+__device__ __forceinline__ float warp_reduce4(const float (&v)[4], int lane, Op op)
+{
+    const bool up = lane & 16, up2 = lane & 8;
+    const float k0 = op(up ? v[2] : v[0], __shfl_xor_sync(~0u, up ? v[0] : v[2], 16));
+    const float k1 = op(up ? v[3] : v[1], __shfl_xor_sync(~0u, up ? v[1] : v[3], 16));
+    float k = op(up2 ? k1 : k0, __shfl_xor_sync(~0u, up2 ? k0 : k1, 8));
+    k = op(k, __shfl_xor_sync(~0u, k, 4));
+    k = op(k, __shfl_xor_sync(~0u, k, 2));
+    return op(k, __shfl_xor_sync(~0u, k, 1));
+}
+
 template <typename OutT, int D, int NH>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(384, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                            const __grid_constant__ PagedArgs a)
 {
@@ -251,20 +293,19 @@ __global__ void __launch_bounds__(256, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_MISC);
-    uint64_t* k_full = bars;               // [8] codes and scales of a stage landed
+    uint64_t* k_full = bars;               // [8] codes (TMA) and scales (cp.async, 32) of a stage landed
     uint64_t* v_full = k_full + 8;         // [8] values landed
     uint64_t* empty = v_full + 8;          // [8] the stage's MMAs are done (commit)
-    uint64_t* sf_full = empty + 8;         // [2] scale atoms written (32)
-    uint64_t* q_full = sf_full + 2;        // [2] query codes and scales written (32)
-    uint64_t* q_empty = q_full + 2;        // [2] the item's S^T MMAs are done (commit)
-    uint64_t* s_full = q_empty + 2;        // [2] S^T computed (commit)
-    uint64_t* s_free = s_full + 2;         // [2] S^T in registers (128)
+    uint64_t* q_full = empty + 8;          // [4] query codes and scales written (32)
+    uint64_t* q_empty = q_full + 4;        // [4] the item's S^T MMAs are done (commit)
+    uint64_t* s_full = q_empty + 4;        // [2][2] S^T computed (commit); by warpgroup, see below
+    uint64_t* s_free = s_full + 4;         // [2] S^T in registers (128)
     uint64_t* p_full = s_free + 2;         // [2] P written (128)
     uint64_t* o_full = p_full + 2;         // [2] O^T computed, P read (commit)
     uint64_t* o_free = o_full + 2;         // [2] O^T in registers (128)
-    uint64_t* drain = o_free + 2;          // everything issued is done (exit)
-    float* red = reinterpret_cast<float*>(smem + C::OFF_MISC + 512);  // [4][NH]
-    int* scratch = reinterpret_cast<int*>(smem + C::OFF_MISC + 1024 + 512);  // [8]
+    uint64_t* drain = o_free + 2;          // [2] everything an issuer issued is done (exit)
+    float* red_all = reinterpret_cast<float*>(smem + C::OFF_MISC + 512);  // [2][4][NH]
+    int* scratch = reinterpret_cast<int*>(smem + C::OFF_MISC + 1536);     // [8]
     PagedRange* range = reinterpret_cast<PagedRange*>(scratch + 8);
     uint32_t* tmem_sh = reinterpret_cast<uint32_t*>(scratch + 16);
     int* abort_sh = scratch + 17;
@@ -272,21 +313,23 @@ __global__ void __launch_bounds__(256, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; i++) {
-            ptx::mbar_init(&k_full[i], 1);
+            ptx::mbar_init(&k_full[i], 1 + 32);
             ptx::mbar_init(&v_full[i], 1);
             ptx::mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; i++) {
-            ptx::mbar_init(&sf_full[i], 32);
+        for (int i = 0; i < C::QBUFS; i++) {
             ptx::mbar_init(&q_full[i], 32);
             ptx::mbar_init(&q_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
             ptx::mbar_init(&s_full[i], 1);
+            ptx::mbar_init(&s_full[2 + i], 1);
             ptx::mbar_init(&s_free[i], 128);
             ptx::mbar_init(&p_full[i], 128);
             ptx::mbar_init(&o_full[i], 1);
             ptx::mbar_init(&o_free[i], 128);
+            ptx::mbar_init(&drain[i], 1);
         }
-        ptx::mbar_init(drain, 1);
         *abort_sh = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tm_k);
@@ -297,10 +340,10 @@ __global__ void __launch_bounds__(256, 1)
         ptx::tmem_relinquish();
     }
     // Query rows past the group's heads and blocks past head_dim: codes 0,
-    // scale 1, for both buffers.
-    for (int i = threadIdx.x; i < 2 * C::Q_BYTES / 16; i += 256)
+    // scale 1, for all buffers.
+    for (int i = threadIdx.x; i < C::QBUFS * C::Q_BYTES / 16; i += C::THREADS)
         reinterpret_cast<uint4*>(smem + C::OFF_Q)[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = threadIdx.x; i < 2 * C::ATOMS * 32; i += 256)
+    for (int i = threadIdx.x; i < C::QBUFS * C::ATOMS * 32; i += C::THREADS)
         reinterpret_cast<uint4*>(smem + C::OFF_QSF)[i] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
     ptx::fence_proxy_async_smem();
     // Everything before this overlaps the grid before this one in the stream.
@@ -313,366 +356,442 @@ __global__ void __launch_bounds__(256, 1)
     const uint32_t tmem = *tmem_sh;
     const int count = range->count;
     const ServingWait w{abort_sh, a.timeout_ns};
-    auto stage_of = [&](int g) { return smem + C::OFF_STAGE + (g % C::STAGES) * C::STAGE; };
-    auto stage_parity = [&](int g) { return static_cast<uint32_t>(g / C::STAGES) & 1u; };
-    auto two_parity = [](int g) { return static_cast<uint32_t>(g / 2) & 1u; };
-    TileWalk t;
+    uint8_t* const stages = smem + C::OFF_STAGE;
+    const int page = a.c.page_size, shift = a.c.page_shift;
+    ItemWalk t;
     t.begin(a, range->start, count);
 
-    if (warp == 0) {
-        // ------------------------------------------------------------ producer
-        const int page = a.c.page_size;
-        int g = 0;
-        for (; t.left > 0; t.next(a), g++) {
-            const int n = (t.keys() + page - 1) >> a.c.page_shift;  // pages of this tile, one per lane (at most 8)
-            int id = 0;
-            if (lane < n) {
-                id = __ldg(a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> a.c.page_shift) + lane);
-                if (id < 0 || id >= a.c.pages) {
-                    record_index_error(kIndexPage, id);
-                    id = 0;
-                }
-            }
-            if (lane == 0 && t.first && t.tile == 0 && t.hg == 0) {
+    if (warp <= 1) {
+        // ------------------------------------------------------------ producers
+        const bool keys_role = warp == 0;
+        Ring<C::STAGES> ring;
+        Ring<C::QBUFS> qr;
+        int g = 0, item = 0;
+        bool ok = true;
+        for (; ok && t.left > 0; t.next(a), item++, qr.next()) {
+            if (keys_role && lane == 0 && t.tile == 0 && t.hg == 0) {
                 const int len = __ldg(a.seq_lens + t.b);
                 if (len != t.len) record_index_error(kIndexLength, len);
             }
-            const int s = g % C::STAGES;
-            if (g >= C::STAGES && !__all_sync(~0u, bounded_wait(&empty[s], stage_parity(g - C::STAGES), w, kPagedEmpty))) break;
-            if (lane == 0) {
-                ptx::mbar_arrive_expect_tx(&k_full[s], n * page * (C::KROW + C::NB));
-                ptx::mbar_arrive_expect_tx(&v_full[s], n * page * D * 2);
+            const int head = t.hg / a.splits;
+            const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift);
+            auto page_id = [&](int i) {  // of this lane's page of the part's i-th tile; 0 past its pages
+                int id = 0;
+                if ((lane << shift) < t.keys(i)) id = __ldg(row + ((i * kPagedTile) >> shift) + lane);
+                return id;
+            };
+            int id = page_id(0);
+            for (int i = 0; i < t.n; i++, g++, ring.next()) {
+                const int next_id = i + 1 < t.n ? page_id(i + 1) : 0;
+                const int n = (t.keys(i) + page - 1) >> shift;  // pages of this tile
+                if (id < 0 || id >= a.c.pages) {
+                    if (keys_role) record_index_error(kIndexPage, id);
+                    id = 0;
+                }
+                uint8_t* st = stages + ring.s * C::STAGE;
+                if (g >= C::STAGES && !__all_sync(~0u, bounded_wait(&empty[ring.s], ring.parity ^ 1u, w, kPagedEmpty))) {
+                    ok = false;
+                    break;
+                }
+                if (keys_role) {
+                    if (lane == 0) ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * C::KROW);
+                    __syncwarp();
+                    if (lane < n) ptx::tma_load_4d(st + lane * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, id);
+                    // Raw scales: 16-byte pieces, page after page.
+                    const int piece_shift = shift - 4;  // log2(page / 16): a page has NB << piece_shift pieces
+#pragma unroll
+                    for (int c0 = 0; c0 < 8 * C::NB; c0 += 32) {
+                        const int c = c0 + lane, p = static_cast<int>(static_cast<unsigned>(c / C::NB) >> piece_shift);
+                        const int pid = __shfl_sync(~0u, id, p & 31);
+                        if (c < 8 * C::NB && p < n)
+                            ptx::cp_async16(st + C::K_BYTES + C::V_BYTES + c * 16,
+                                            a.c.k_scales + pid * a.c.k_scales_stride +
+                                                static_cast<int64_t>(head) * page * C::NB + (c * 16 - p * page * C::NB));
+                    }
+                    ptx::cp_async_arrive(&k_full[ring.s]);
+                } else {
+                    if (lane == 0) ptx::mbar_arrive_expect_tx(&v_full[ring.s], n * page * D * 2);
+                    __syncwarp();
+                    if (lane < n) ptx::tma_load_5d(st + C::K_BYTES + lane * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, id);
+                }
+                __syncwarp();
+                id = next_id;
+                if (keys_role || i > 0) continue;
+                // This item's queries.
+                if (item >= C::QBUFS && !__all_sync(~0u, bounded_wait(&q_empty[qr.s], qr.parity ^ 1u, w, kPagedQEmpty))) {
+                    ok = false;
+                    g++;  // (the tile just issued is in flight)
+                    break;
+                }
+                const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
+                const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(head) * a.group + h0) * a.qh;
+                for (int k = lane; k < nh * C::NB; k += 32) {
+                    const int r = k / C::NB, blk = k % C::NB;
+                    const int64_t at = q0 + r * a.qh + blk * 32;
+                    uint4 packed;
+                    uint32_t sb = a.q_half ? quantize32<__half>(static_cast<const __half*>(a.q) + at, a.ocp, packed)
+                                           : quantize32<float>(static_cast<const float*>(a.q) + at, a.ocp, packed);
+                    if (sb == 255u) sb = 254u;
+                    const int sw = C::KROW == 32 ? (r >> 2) & 1 : C::KROW == 64 ? (r >> 1) & 3 : r & 7;
+                    *reinterpret_cast<uint4*>(smem + C::OFF_Q + qr.s * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16)) = packed;
+                    smem[C::OFF_QSF + (qr.s * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb);
+                }
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(&q_full[qr.s]);
             }
-            __syncwarp();
-            if (lane < n) {
-                uint8_t* st = stage_of(g);
-                const int head = t.hg / a.splits;
-                ptx::tma_load_4d(st + lane * page * C::KROW, &tm_k, &k_full[s], 0, head, id);
-                ptx::bulk_load(st + C::K_BYTES + C::V_BYTES + lane * page * C::NB,
-                               a.c.k_scales + id * a.c.k_scales_stride + static_cast<int64_t>(head) * page * C::NB,
-                               page * C::NB, &k_full[s]);
-                ptx::tma_load_5d(st + C::K_BYTES + lane * page * D * 2, &tm_v, &v_full[s], 0, 0, head, id);
-            }
-            __syncwarp();
         }
         // Every copy issued lands before the block exits.
+        ptx::cp_async_wait_all();
         if (lane == 0)
-            for (int i = max(0, g - C::STAGES); i < g; i++) {
-                bounded_drain(&k_full[i % C::STAGES], stage_parity(i), 2 * a.timeout_ns);
-                bounded_drain(&v_full[i % C::STAGES], stage_parity(i), 2 * a.timeout_ns);
-            }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t qk_sw = ptx::swizzle_mode_for_bytes(C::KROW);
-            constexpr uint32_t idesc_o = ptx::idesc_f16x(128, NH, 0, true, true);
-            int item = -1;
-            auto issue_s = [&](const TileWalk& x, int g) {
-                const int s = g % C::STAGES, buf = g & 1;
-                if (x.first) {
-                    item++;
-                    if (!bounded_wait(&q_full[item & 1], two_parity(item), w, kPagedQFull)) return false;
-                }
-                if (!bounded_wait(&k_full[s], stage_parity(g), w, kPagedKFull)) return false;
-                if (!bounded_wait(&sf_full[buf], two_parity(g), w, kPagedScales)) return false;
-                if (g >= 2 && !bounded_wait(&s_free[buf], two_parity(g - 2), w, kPagedSFree)) return false;
-                ptx::tc_fence_after();
-                if (x.first)
-#pragma unroll
-                    for (int i = 0; i < C::ATOMS; i++)
-                        ptx::tc_cp_32x128b_warpx4(tmem + C::SFB_COL + 4 * i,
-                                                  ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_QSF + ((item & 1) * C::ATOMS + i) * 512),
-                                                                  0, 128, ptx::kSwizzleNone));
-#pragma unroll
-                for (int i = 0; i < C::ATOMS; i++)
-                    ptx::tc_cp_32x128b_warpx4(tmem + C::SFA_COL + 4 * i,
-                                              ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_KSF + (buf * C::ATOMS + i) * 512), 0,
-                                                              128, ptx::kSwizzleNone));
-                const uint64_t kd = ptx::make_sdesc(ptx::smem_u32(stage_of(g)), 16, 8 * C::KROW, qk_sw);
-                const uint64_t qd = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_Q + (item & 1) * C::Q_BYTES), 16, 8 * C::KROW, qk_sw);
-#pragma unroll
-                for (int kk = 0; kk < C::KSTEPS; kk++) {
-                    const uint32_t id = 2u * (kk & 1);
-                    ptx::mma_mxf4(tmem + C::S_COL + buf * NH, kd + 2 * kk, qd + 2 * kk, ptx::idesc_mxf4(128, NH, id, id),
-                                  (tmem + C::SFA_COL + 4 * (kk / 2)) | (id << 30),
-                                  (tmem + C::SFB_COL + 4 * (kk / 2)) | (id << 30), kk > 0 ? 1u : 0u);
-                }
-                ptx::tc_commit(&s_full[buf]);
-                if (x.last()) ptx::tc_commit(&q_empty[item & 1]);
-                return true;
-            };
-            const int page = a.c.page_size;
-            auto issue_o = [&](const TileWalk& x, int g) {
-                const int s = g % C::STAGES, buf = g & 1;
-                if (!bounded_wait(&v_full[s], stage_parity(g), w, kPagedVFull)) return false;
-                if (!bounded_wait(&p_full[buf], two_parity(g), w, kPagedPFull)) return false;
-                if (g >= 2 && !bounded_wait(&o_free[buf], two_parity(g - 2), w, kPagedOFree)) return false;
-                ptx::tc_fence_after();
-                const int steps = max(1, (x.keys() + 15) / 16);
-                const uint32_t v0 = ptx::smem_u32(stage_of(g) + C::K_BYTES);
-                for (int kk = 0; kk < steps; kk++) {
-                    const int row = kk * 16, pg = row >> a.c.page_shift;
-                    const uint32_t at = v0 + pg * page * D * 2 + (row & (page - 1)) * C::CB;
-#pragma unroll
-                    for (int part = 0; part < C::PARTS; part++) {
-                        const uint64_t pd = ptx::make_sdesc(
-                            ptx::smem_u32(smem + C::OFF_P + (buf * C::PARTS + part) * C::P_BYTES) + row * C::PROW,
-                            C::P_BYTES, 8 * C::PROW, C::PSW);
-#pragma unroll
-                        for (int m = 0; m < C::MT; m++)
-                            ptx::mma_f16_ss(tmem + C::O_COL + (buf * C::MT + m) * NH,
-                                            ptx::make_sdesc(at + m * (128 / C::CHE) * page * C::CB, page * C::CB, 8 * C::CB, C::VSW),
-                                            pd, idesc_o, (kk > 0 || part > 0) ? 1u : 0u);
-                    }
-                }
-                ptx::tc_commit(&o_full[buf]);
-                ptx::tc_commit(&empty[s]);
-                return true;
-            };
-            TileWalk o = t;
-            int gs = 0, go = 0;
-            bool ok = true;
-            if (t.left > 0) {
-                ok = issue_s(t, gs++);
-                t.next(a);
-            }
-            while (ok && o.left > 0) {
-                if (t.left > 0) {
-                    if (!(ok = issue_s(t, gs++))) break;
-                    t.next(a);
-                }
-                ok = issue_o(o, go++);
-                o.next(a);
-            }
-            // Everything issued completes before Tensor Memory is freed.
-            ptx::tc_commit(drain);
-            bounded_drain(drain, 0, 2 * a.timeout_ns);
-        }
+            for (int i = max(0, g - C::STAGES); i < g; i++)
+                bounded_drain(keys_role ? &k_full[i % C::STAGES] : &v_full[i % C::STAGES],
+                              static_cast<uint32_t>(i / C::STAGES) & 1u, 2 * a.timeout_ns);
         __syncwarp();
     } else if (warp == 2) {
-        // ------------------------------------------------------------ scales
-        // Lane l writes row l of each atom: the scales of keys l, 32 + l, 64 + l, 96 + l.
-        for (int g = 0; t.left > 0; t.next(a), g++) {
-            const int buf = g & 1;
-            if (!__all_sync(~0u, bounded_wait(&k_full[g % C::STAGES], stage_parity(g), w, kPagedKFull))) break;
-            // (the S^T MMAs of tile g - 2 have read this atom buffer)
-            if (g >= 2 && !__all_sync(~0u, bounded_wait(&s_full[buf], two_parity(g - 2), w, kPagedSFull))) break;
-            const uint8_t* raw = stage_of(g) + C::K_BYTES + C::V_BYTES;
-#pragma unroll
-            for (int i = 0; i < C::ATOMS; i++) {
-                uint32_t word[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint8_t* p = raw + (c * 32 + lane) * C::NB + 4 * i;
-                    if constexpr (C::NB % 4 == 0) {
-                        word[c] = *reinterpret_cast<const uint32_t*>(p);
-                    } else {
-                        word[c] = 0u;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) word[c] |= (4 * i + j < C::NB ? p[j] : 127u) << (8 * j);
-                    }
+        // ------------------------------------------------------------ S^T issuer
+        constexpr uint32_t qk_sw = ptx::swizzle_mode_for_bytes(C::KROW);
+        const uint64_t kd0 = ptx::make_sdesc(ptx::smem_u32(stages), 16, 8 * C::KROW, qk_sw);
+        const uint64_t qd0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_Q), 16, 8 * C::KROW, qk_sw);
+        const uint64_t sfa0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_KSF), 0, 128, ptx::kSwizzleNone);
+        const uint64_t sfb0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_QSF), 0, 128, ptx::kSwizzleNone);
+        Ring<C::STAGES> ring;
+        Ring<C::QBUFS> qr;
+        // A warpgroup waits for its own tiles only, and a barrier's parity tells
+        // a phase from the one before it alone: so each has its own barriers,
+        // used in the order of its tiles.
+        int g = 0, own[2] = {0, 0};
+        bool ok = true;
+        for (int wg = 0; ok && t.left > 0; t.next(a), qr.next(), wg ^= 1) {
+            const int qb = qr.s;
+            int j = own[wg];
+            own[wg] += t.n;
+            for (int i = 0; i < t.n; i++, g++, j++, ring.next()) {
+                const int buf = g & 1;
+                // S^T and the scale atoms of tile g - 2 have been read.
+                bool go = g < 2 || bounded_wait(&s_free[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedSFree);
+                go = bounded_wait(&k_full[ring.s], ring.parity, w, kPagedKFull) && go;
+                if (i == 0) go = bounded_wait(&q_full[qb], qr.parity, w, kPagedQFull) && go;
+                if (!__all_sync(~0u, go)) {
+                    ok = false;
+                    break;
                 }
-                *reinterpret_cast<uint4*>(smem + C::OFF_KSF + (buf * C::ATOMS + i) * 512 + lane * 16) =
-                    make_uint4(word[0], word[1], word[2], word[3]);
+                // Lane l writes row l of each atom: the scales of keys l, 32 + l, 64 + l, 96 + l.
+                const uint8_t* raw = stages + ring.s * C::STAGE + C::K_BYTES + C::V_BYTES;
+#pragma unroll
+                for (int k = 0; k < C::ATOMS; k++) {
+                    uint32_t word[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint8_t* p = raw + (c * 32 + lane) * C::NB + 4 * k;
+                        if constexpr (C::NB % 4 == 0) {
+                            word[c] = *reinterpret_cast<const uint32_t*>(p);
+                        } else {
+                            word[c] = 0u;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) word[c] |= (4 * k + j < C::NB ? p[j] : 127u) << (8 * j);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(smem + C::OFF_KSF + (buf * C::ATOMS + k) * 512 + lane * 16) =
+                        make_uint4(word[0], word[1], word[2], word[3]);
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::tc_fence_after();
+                    if (i == 0)
+#pragma unroll
+                        for (int k = 0; k < C::ATOMS; k++)
+                            ptx::tc_cp_32x128b_warpx4(tmem + C::SFB_COL + 4 * k, sfb0 + (qb * C::ATOMS + k) * (512 / 16));
+#pragma unroll
+                    for (int k = 0; k < C::ATOMS; k++)
+                        ptx::tc_cp_32x128b_warpx4(tmem + C::SFA_COL + 4 * k, sfa0 + (buf * C::ATOMS + k) * (512 / 16));
+                    const uint64_t kd = kd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16)), qd = qd0 + qb * (C::Q_BYTES / 16);
+#pragma unroll
+                    for (int kk = 0; kk < C::KSTEPS; kk++) {
+                        const uint32_t id = 2u * (kk & 1);
+                        ptx::mma_mxf4(tmem + C::S_COL + buf * NH, kd + 2 * kk, qd + 2 * kk, ptx::idesc_mxf4(128, NH, id, id),
+                                      (tmem + C::SFA_COL + 4 * (kk / 2)) | (id << 30),
+                                      (tmem + C::SFB_COL + 4 * (kk / 2)) | (id << 30), kk > 0 ? 1u : 0u);
+                    }
+                    ptx::tc_commit(&s_full[2 * wg + (j & 1)]);
+                    if (i + 1 == t.n) ptx::tc_commit(&q_empty[qb]);
+                }
+                __syncwarp();
             }
-            ptx::fence_proxy_async_smem();
-            ptx::mbar_arrive(&sf_full[buf]);
         }
+        if (lane == 0) {  // everything issued completes before Tensor Memory is freed
+            ptx::tc_commit(&drain[0]);
+            bounded_drain(&drain[0], 0, 2 * a.timeout_ns);
+        }
+        __syncwarp();
     } else if (warp == 3) {
-        // ------------------------------------------------------------ queries
-        int item = 0;
-        for (; t.left > 0; t.next(a)) {
-            if (!t.first) continue;
-            const int buf = item & 1;
-            if (item >= 2 && !__all_sync(~0u, bounded_wait(&q_empty[buf], two_parity(item - 2), w, kPagedQEmpty))) break;
-            const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
-            const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(t.hg / a.splits) * a.group + h0) * a.qh;
-            for (int i = lane; i < nh * C::NB; i += 32) {
-                const int r = i / C::NB, blk = i % C::NB;
-                uint4 packed;
-                const int64_t at = q0 + r * a.qh + blk * 32;
-                uint32_t sb = a.q_half ? quantize32<__half>(static_cast<const __half*>(a.q) + at, a.ocp, packed)
-                                       : quantize32<float>(static_cast<const float*>(a.q) + at, a.ocp, packed);
-                if (sb == 255u) sb = 254u;
-                const int sw = C::KROW == 32 ? (r >> 2) & 1 : C::KROW == 64 ? (r >> 1) & 3 : r & 7;
-                *reinterpret_cast<uint4*>(smem + C::OFF_Q + buf * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16)) = packed;
-                smem[C::OFF_QSF + (buf * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb);
+        // ------------------------------------------------------------ O^T issuer
+        if (lane == 0) {
+            constexpr uint32_t idesc_o = ptx::idesc_f16x(128, NH, 0, true, true);
+            // V's 16-key steps within a stage (in 16-byte units): page by page, rows within a page.
+            uint64_t vo[8];
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++)
+                vo[kk] = static_cast<uint64_t>((((kk * 16) >> shift) * page * D * 2 + ((kk * 16) & (page - 1)) * C::CB) >> 4);
+            const uint64_t vd0 = ptx::make_sdesc(ptx::smem_u32(stages + C::K_BYTES), page * C::CB, 8 * C::CB, C::VSW);
+            const uint64_t pd0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_P), C::P_BYTES, 8 * C::PROW, C::PSW);
+            const uint64_t m_step = static_cast<uint64_t>((128 / C::CHE) * page * C::CB / 16);
+            Ring<C::STAGES> ring;
+            int g = 0;
+            bool ok = true;
+            for (; ok && t.left > 0; t.next(a)) {
+                for (int i = 0; i < t.n; i++, g++, ring.next()) {
+                    const int buf = g & 1;
+                    const int steps = max(1, (t.keys(i) + 15) / 16);
+                    const uint64_t vd = vd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16));
+                    const uint64_t pd = pd0 + static_cast<uint64_t>(buf * C::PARTS * C::P_BYTES / 16);
+                    const uint32_t od = tmem + C::O_COL + buf * C::MT * NH;
+                    ok = (g < 2 || bounded_wait(&o_free[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedOFree)) &&
+                         bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull) &&
+                         bounded_wait(&p_full[buf], static_cast<uint32_t>(g / 2) & 1u, w, kPagedPFull);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < 8; kk++) {
+                        if (kk >= steps) break;
+#pragma unroll
+                        for (int part = 0; part < C::PARTS; part++)
+#pragma unroll
+                            for (int m = 0; m < C::MT; m++)
+                                ptx::mma_f16_ss(od + m * NH, vd + vo[kk] + m * m_step,
+                                                pd + (part * C::P_BYTES + kk * 16 * C::PROW) / 16, idesc_o,
+                                                (kk > 0 || part > 0) ? 1u : 0u);
+                    }
+                    ptx::tc_commit(&o_full[buf]);
+                    ptx::tc_commit(&empty[ring.s]);
+                }
             }
-            ptx::fence_proxy_async_smem();
-            ptx::mbar_arrive(&q_full[buf]);
-            item++;
+            ptx::tc_commit(&drain[1]);
+            bounded_drain(&drain[1], 0, 2 * a.timeout_ns);
         }
+        __syncwarp();
     } else {
         // ------------------------------------------------------------ softmax
-        const int wq = warp - 4, row = wq * 32 + lane;  // key of the tile; head-dim row of O^T
+        const int wg = (warp - 4) / 4, wq = warp % 4, row = wq * 32 + lane;  // key of the tile; head-dim row of O^T
         const uint32_t lanes = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+        const int bar_id = 1 + wg;
+        float* red = red_all + wg * 4 * NH;
         constexpr float kGrowth = 8.f;  // how far (log2) a score may exceed the reference
-        float m[NH], l[NH], o[C::MT][NH];
+        constexpr int CH = NH / 4;      // heads in fours: fours past the group's heads are skipped
+        float nm[NH], l[NH], o[C::MT][NH];  // minus the reference, this thread's sums, O^T
         bool ok = true;  // no wait of this thread has run out
         auto load_cols = [&](uint32_t col, uint32_t (&r)[NH]) {
             if constexpr (NH == 16) ptx::tmem_ld16(lanes + col, r);
             else ptx::tmem_ld32(lanes + col, r);
         };
-        // Adds tile g's O^T to the registers.
-        auto add_o = [&](int g) {
-            const int buf = g & 1;
-            if (!__all_sync(~0u, bounded_wait(&o_full[buf], two_parity(g), w, kPagedOFull))) {
-                ok = false;
-                return;
+        auto max_of = [](float x, float y) { return fmaxf(x, y); };
+        auto sum_of = [](float x, float y) { return x + y; };
+        Ring<C::STAGES> ring;
+        int g = 0, j = 0;  // tile of the block, tile of this warpgroup
+        for (int item = 0; t.left > 0; t.next(a), item++) {
+            if ((item & 1) != wg) {  // the other warpgroup's
+                g += t.n;
+                for (int i = t.n % C::STAGES; i > 0; i--) ring.next();
+                ring.parity ^= static_cast<uint32_t>(t.n / C::STAGES) & 1u;
+                continue;
             }
-            ptx::tc_fence_after();
-            uint32_t r[C::MT][NH];
-#pragma unroll
-            for (int i = 0; i < C::MT; i++) load_cols(C::O_COL + (buf * C::MT + i) * NH, r[i]);
-            ptx::tc_wait_ld();
-            ptx::tc_fence_before();
-            ptx::mbar_arrive(&o_free[buf]);
-#pragma unroll
-            for (int i = 0; i < C::MT; i++)
-#pragma unroll
-                for (int h = 0; h < NH; h++) o[i][h] += __uint_as_float(r[i][h]);
-        };
-        int g = 0;
-        bool pending = false;  // tile g - 1's O^T is not yet added
-        for (; t.left > 0; t.next(a), g++) {
-            const int buf = g & 1, n = t.keys();
             const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
-            if (t.first) {
-#pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    m[h] = -INFINITY;
-                    l[h] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < C::MT; i++) o[i][h] = 0.f;
+            // Adds tile g's O^T to the registers.
+            auto add_o = [&](int tile_g) {
+                const int buf = tile_g & 1;
+                if (!__all_sync(~0u, bounded_wait(&o_full[buf], static_cast<uint32_t>(tile_g / 2) & 1u, w, kPagedOFull))) {
+                    ok = false;
+                    return;
                 }
-            }
-            ok = __all_sync(~0u, bounded_wait(&s_full[buf], two_parity(g), w, kPagedSFull)) && ok;
-            ptx::tc_fence_after();
-            uint32_t sr[NH];
-            load_cols(C::S_COL + buf * NH, sr);
-            ptx::tc_wait_ld();
-            ptx::tc_fence_before();
-            ptx::mbar_arrive(&s_free[buf]);
-            float x[NH];
-            bool over = t.first || !ok;
+                ptx::tc_fence_after();
+                uint32_t r[C::MT][NH];
 #pragma unroll
-            for (int h = 0; h < NH; h++) {
-                x[h] = row < n ? __uint_as_float(sr[h]) * a.scale_log2 : -INFINITY;
-                over |= h < nh && x[h] > m[h] + kGrowth;
-            }
-            if (ptx::named_bar_any(1, 128, over)) {
-                // Rare: a new item, a score that outgrew the reference, or a
-                // wait that ran out.  All 128 threads come here together.
-                if (ptx::named_bar_any(1, 128, !ok)) break;
-                if (pending) {
-                    add_o(g - 1);
-                    pending = false;
+                for (int m = 0; m < C::MT; m++) load_cols(C::O_COL + (buf * C::MT + m) * NH, r[m]);
+                ptx::tc_wait_ld();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(&o_free[buf]);
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+                    if (4 * c < nh)
+#pragma unroll
+                        for (int m = 0; m < C::MT; m++)
+#pragma unroll
+                            for (int h = 4 * c; h < 4 * c + 4; h++) o[m][h] += __uint_as_float(r[m][h]);
+            };
+            bool pending = false, out_of_time = false;  // pending: tile g - 1's O^T is not yet added
+            for (int i = 0; i < t.n; i++, g++, j++, ring.next()) {
+                const int buf = g & 1, n = t.keys(i);
+                ok = __all_sync(~0u, bounded_wait(&s_full[2 * wg + (j & 1)], static_cast<uint32_t>(j / 2) & 1u, w, kPagedSFull)) && ok;
+                ptx::tc_fence_after();
+                uint32_t sr[NH];
+                load_cols(C::S_COL + buf * NH, sr);
+                ptx::tc_wait_ld();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(&s_free[buf]);
+                float x[NH];  // the scores, log2 domain, less the reference
+                bool over = i == 0 || !ok;
+                if (n < kPagedTile)
+#pragma unroll
+                    for (int h = 0; h < NH; h++)
+                        if (row >= n) sr[h] = 0xFF800000u;  // -inf
+                if (i == 0) {
+#pragma unroll
+                    for (int h = 0; h < NH; h++) nm[h] = 0.f;
                 }
 #pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    const float v = ptx::warp_max(x[h]);
-                    if (lane == 0) red[wq * NH + h] = v;
+                for (int c = 0; c < CH; c++)
+                    if (4 * c < nh)
+#pragma unroll
+                        for (int h = 4 * c; h < 4 * c + 4; h++) {
+                            x[h] = fmaf(__uint_as_float(sr[h]), a.scale_log2, nm[h]);
+                            over |= x[h] > kGrowth;
+                        }
+                if (ptx::named_bar_any(bar_id, 128, over)) {
+                    // Rare: a new item, a score that outgrew the reference, or
+                    // a wait that ran out.  All 128 threads come here together.
+                    if (ptx::named_bar_any(bar_id, 128, !ok)) {
+                        out_of_time = true;
+                        break;
+                    }
+                    if (pending) {
+                        add_o(g - 1);
+                        pending = false;
+                    }
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+                        if (4 * c < nh) {
+                            const float v[4] = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+                            const float top = warp_reduce4(v, lane, max_of);
+                            if ((lane & 7) == 0) red[wq * NH + 4 * c + (lane >> 3)] = top;
+                        }
+                    ptx::named_bar_sync(bar_id, 128);
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+                        if (4 * c < nh) {
+                            float top[4];
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const float4 f = *reinterpret_cast<const float4*>(red + q * NH + 4 * c);
+                                top[0] = q ? fmaxf(top[0], f.x) : f.x;
+                                top[1] = q ? fmaxf(top[1], f.y) : f.y;
+                                top[2] = q ? fmaxf(top[2], f.z) : f.z;
+                                top[3] = q ? fmaxf(top[3], f.w) : f.w;
+                            }
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                // How far the reference moves: up, or at an item's start to the maximum (0
+                                // when there is no key at all).
+                                const int h = 4 * c + q;
+                                const float up = i > 0 ? fmaxf(top[q], 0.f) : top[q] == -INFINITY ? 0.f : top[q];
+                                const float alpha = i > 0 ? ptx::ex2_approx(-up) : 0.f;
+                                nm[h] -= up;
+                                x[h] -= up;
+                                l[h] = i > 0 ? l[h] * alpha : 0.f;
+#pragma unroll
+                                for (int m = 0; m < C::MT; m++) o[m][h] = i > 0 ? o[m][h] * alpha : 0.f;
+                            }
+                        }
                 }
-                ptx::named_bar_sync(1, 128);
+                // P of this key.  Its buffer was last read by tile g - 2's O^T:
+                // added above, unless the other warpgroup had it.  (Tile g - 4's
+                // is complete then, so the parity is unambiguous: if it was the
+                // other warpgroup's, that added it before it read S^T of g - 2.)
+                if (i < 2 && g >= 2)
+                    ok = __all_sync(~0u, bounded_wait(&o_full[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedOFull)) && ok;
+                uint8_t* p = smem + C::OFF_P + buf * C::PARTS * C::P_BYTES + row * C::PROW;
+                const int sw = C::PROW == 32 ? (row >> 2) & 1 : (row >> 1) & 3;
 #pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    const float top = fmaxf(fmaxf(red[h], red[NH + h]), fmaxf(red[2 * NH + h], red[3 * NH + h]));
-                    const float to = fmaxf(m[h], top);
-                    const float alpha = m[h] == -INFINITY ? 0.f : ptx::ex2_approx(m[h] - to);
-                    m[h] = to;
-                    l[h] *= alpha;
+                for (int u = 0; u < NH / 8; u++) {
+                    if (8 * u >= nh) break;
+                    uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-                    for (int i = 0; i < C::MT; i++) o[i][h] *= alpha;
+                    for (int c = 2 * u; c < 2 * u + 2; c++)
+                        if (4 * c < nh)
+#pragma unroll
+                            for (int h = 4 * c; h < 4 * c + 4; h += 2) {
+                                const float p0 = ptx::ex2_approx(x[h]), p1 = ptx::ex2_approx(x[h + 1]);
+                                l[h] += p0;
+                                l[h + 1] += p1;
+                                const uint32_t pk = ptx::pack_half2(p0, p1);
+                                hi[(h - 8 * u) / 2] = pk;
+                                if constexpr (kSplitP) {
+                                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pk));
+                                    lo[(h - 8 * u) / 2] = ptx::pack_half2(p0 - f.x, p1 - f.y);
+                                }
+                            }
+                    *reinterpret_cast<uint4*>(p + ((u ^ sw) * 16)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (kSplitP)
+                        *reinterpret_cast<uint4*>(p + C::P_BYTES + ((u ^ sw) * 16)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
-                ptx::named_bar_sync(1, 128);  // (red is written again at the item's end)
-            }
-            // P of this key.  Its buffer was last read by tile g - 2's O^T, which is added.
-            uint32_t ph[NH / 2], pl[NH / 2];
+                if (row >= n && row < max(16, (n + 15) / 16 * 16)) {
+                    // A key behind the last: whatever lies in its place of V
+                    // (NaN included) must not meet its weight of zero.
+                    ok = bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull) && ok;
+                    uint8_t* v = stages + ring.s * C::STAGE + C::K_BYTES + (row >> shift) * page * D * 2 + (row & (page - 1)) * C::CB;
+                    for (int c = 0; c < C::DCH; c++)
 #pragma unroll
-            for (int h = 0; h < NH; h += 2) {
-                const float p0 = ptx::ex2_approx(x[h] - (m[h] == -INFINITY ? 0.f : m[h]));
-                const float p1 = ptx::ex2_approx(x[h + 1] - (m[h + 1] == -INFINITY ? 0.f : m[h + 1]));
-                l[h] += p0;
-                l[h + 1] += p1;
-                ph[h / 2] = ptx::pack_half2(p0, p1);
-                if constexpr (kSplitP) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ph[h / 2]));
-                    pl[h / 2] = ptx::pack_half2(p0 - f.x, p1 - f.y);
+                        for (int u = 0; u < C::CB / 16; u++)
+                            *reinterpret_cast<uint4*>(v + c * page * C::CB + u * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
+                __syncwarp();
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(&p_full[buf]);
+                if (pending) add_o(g - 1);
+                pending = true;
             }
-            uint8_t* p = smem + C::OFF_P + buf * C::PARTS * C::P_BYTES + row * C::PROW;
-            const int sw = C::PROW == 32 ? (row >> 2) & 1 : (row >> 1) & 3;
+            if (out_of_time) break;
+            // The item's end in this block: g is one past its last tile here.
 #pragma unroll
-            for (int u = 0; u < NH / 8; u++) {
-                *reinterpret_cast<uint4*>(p + ((u ^ sw) * 16)) = make_uint4(ph[4 * u], ph[4 * u + 1], ph[4 * u + 2], ph[4 * u + 3]);
-                if constexpr (kSplitP)
-                    *reinterpret_cast<uint4*>(p + C::P_BYTES + ((u ^ sw) * 16)) =
-                        make_uint4(pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]);
-            }
-            if (row >= n && row < max(16, (n + 15) / 16 * 16)) {
-                // A key behind the last: whatever lies in its place of V (NaN
-                // included) must not meet its weight of zero.
-                ok = bounded_wait(&v_full[g % C::STAGES], stage_parity(g), w, kPagedVFull) && ok;
-                const int page = a.c.page_size;
-                uint8_t* v = stage_of(g) + C::K_BYTES + (row >> a.c.page_shift) * page * D * 2 + (row & (page - 1)) * C::CB;
-                for (int c = 0; c < C::DCH; c++)
+            for (int c = 0; c < CH; c++)
+                if (4 * c < nh) {
+                    const float v[4] = {l[4 * c], l[4 * c + 1], l[4 * c + 2], l[4 * c + 3]};
+                    const float sum = warp_reduce4(v, lane, sum_of);
+                    if ((lane & 7) == 0) red[wq * NH + 4 * c + (lane >> 3)] = sum;
+                }
+            ptx::named_bar_sync(bar_id, 128);
+            add_o(g - 1);
+            const bool begun = t.tile == 0;  // the item's first tile is in the range
+            const bool whole = begun && t.n == t.tiles;
+            const int slot = 2 * blockIdx.x + (t.left < count ? 1 : 0);
+            const int64_t o0 = static_cast<int64_t>(t.b) * a.q_heads + (t.hg / a.splits) * a.group + h0;
 #pragma unroll
-                    for (int u = 0; u < C::CB / 16; u++)
-                        *reinterpret_cast<uint4*>(v + c * page * C::CB + u * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            __syncwarp();
-            ptx::fence_proxy_async_smem();
-            ptx::mbar_arrive(&p_full[buf]);
-            if (pending) add_o(g - 1);
-            pending = true;
-            if (!t.last()) continue;
-            // The item's end in this block.
-            add_o(g);
-            pending = false;
+            for (int c = 0; c < CH; c++) {
+                if (4 * c >= nh) break;
+                float sum[4];
 #pragma unroll
-            for (int h = 0; h < NH; h++) {
-                float v = l[h];
+                for (int q = 0; q < 4; q++) {
+                    const float4 f = *reinterpret_cast<const float4*>(red + q * NH + 4 * c);
+                    sum[0] = q ? sum[0] + f.x : f.x;
+                    sum[1] = q ? sum[1] + f.y : f.y;
+                    sum[2] = q ? sum[2] + f.z : f.z;
+                    sum[3] = q ? sum[3] + f.w : f.w;
+                }
 #pragma unroll
-                for (int i = 16; i; i >>= 1) v += __shfl_xor_sync(~0u, v, i);
-                if (lane == 0) red[wq * NH + h] = v;
-            }
-            ptx::named_bar_sync(1, 128);
-#pragma unroll
-            for (int h = 0; h < NH; h++) l[h] = (red[h] + red[NH + h]) + (red[2 * NH + h] + red[3 * NH + h]);
-            const int at = count - t.left;          // this tile's place in the range
-            const bool begun = t.tile <= at;        // the item's first tile is in the range
-            const bool whole = begun && t.tile + 1 == t.tiles;
-            const int slot = 2 * blockIdx.x + (t.tile < at ? 1 : 0);
-            if (whole) {
-                const int64_t o0 = static_cast<int64_t>(t.b) * a.q_heads + (t.hg / a.splits) * a.group + h0;
-#pragma unroll
-                for (int h = 0; h < NH; h++) {
+                for (int q = 0; q < 4; q++) {
+                    const int h = 4 * c + q;
                     if (h >= nh) break;
-                    const float inv = l[h] > 0.f ? 1.0f / l[h] : 0.f;
+                    if (whole) {
+                        const float inv = sum[q] > 0.f ? 1.0f / sum[q] : 0.f;
 #pragma unroll
-                    for (int i = 0; i < C::MT; i++)
-                        if (i * 128 + row < D)
-                            static_cast<OutT*>(a.out)[(o0 + h) * D + i * 128 + row] = from_float<OutT>(o[i][h] * inv);
-                    if (a.lse && row == h)
-                        a.lse[o0 + h] = l[h] > 0.f ? (m[h] + log2f(l[h])) * 0.6931471805599453f : INFINITY;
-                }
-            } else {
-                float* po = a.p.o + static_cast<int64_t>(slot) * NH * D;
+                        for (int m = 0; m < C::MT; m++)
+                            if (m * 128 + row < D)
+                                static_cast<OutT*>(a.out)[(o0 + h) * D + m * 128 + row] = from_float<OutT>(o[m][h] * inv);
+                        if (a.lse && row == h)
+                            a.lse[o0 + h] = sum[q] > 0.f ? (log2f(sum[q]) - nm[h]) * 0.6931471805599453f : INFINITY;
+                    } else {
 #pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    if (h >= nh) break;
-#pragma unroll
-                    for (int i = 0; i < C::MT; i++)
-                        if (i * 128 + row < D) po[h * D + i * 128 + row] = o[i][h];
-                    if (row == h) a.p.ml[slot * NH + h] = make_float2(m[h], l[h]);
+                        for (int m = 0; m < C::MT; m++)
+                            if (m * 128 + row < D)
+                                a.p.o[(static_cast<int64_t>(slot) * NH + h) * D + m * 128 + row] = o[m][h];
+                        if (row == h) a.p.ml[slot * NH + h] = make_float2(-nm[h], sum[q]);
+                    }
                 }
             }
-            if (row == 0 && t.left == 1) {
+            if (row == 0 && t.left == t.n) {
                 // What the join has to do for this block: the item begun here that goes on.
                 int4 it = make_int4(-1, 0, 0, 0);
                 if (begun && !whole) {
-                    const int64_t total = range->total, last = range->first + at + (t.tiles - 1 - t.tile);  // its last tile
+                    const int64_t total = range->total, last = range->first + count - t.n + t.tiles - 1;  // its last tile
                     int c = static_cast<int>(last * range->blocks / total);
                     while (c + 1 < range->blocks && paged_first(total, c + 1, range->blocks) <= last) c++;
                     while (paged_first(total, c, range->blocks) > last) c--;
@@ -680,7 +799,7 @@ __global__ void __launch_bounds__(256, 1)
                 }
                 a.p.items[blockIdx.x] = it;
             }
-            ptx::named_bar_sync(1, 128);  // (red is free again)
+            ptx::named_bar_sync(bar_id, 128);  // (red is free again)
         }
         if (count == 0 && threadIdx.x == 128) a.p.items[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
