@@ -176,9 +176,8 @@ int encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* b
     return r == CUDA_SUCCESS ? FP4ATTN_OK : fail(FP4ATTN_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
 }
 
-// Query heads the attention's MMAs take at once, and the groups a key/value
-// head's query heads are split into.
-int mma_heads(int group) { return group <= 16 ? 16 : 32; }
+// Query heads of a group computed at once (a larger group is split).
+int heads_at_once(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : group <= 16 ? 16 : 32; }
 
 struct AttentionWorkspace {
     size_t items, ml, o, total;
@@ -186,7 +185,7 @@ struct AttentionWorkspace {
 
 AttentionWorkspace attention_workspace(int group, int head_dim)
 {
-    const size_t rows = static_cast<size_t>(2 * kPagedBlocks) * mma_heads(group);
+    const size_t rows = static_cast<size_t>(2 * kPagedBlocks) * heads_at_once(group);
     AttentionWorkspace w{};
     w.ml = (kPagedBlocks * sizeof(int4) + 255) / 256 * 256;
     w.o = w.ml + rows * sizeof(float2);
@@ -211,11 +210,11 @@ int launch_after(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem,
     return FP4ATTN_OK;
 }
 
-template <typename OutT, int D, int NH>
+template <typename OutT, int D, int HC>
 int launch_attention(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
 {
-    using C = PagedCfg<D, NH, sizeof(OutT) == 4>;
-    auto kern = paged_attention_kernel<OutT, D, NH>;
+    using C = PagedCfg<D, HC, sizeof(OutT) == 4>;
+    auto kern = paged_attention_kernel<OutT, D, HC>;
     // The shared memory limit is an attribute of the kernel in a context.
     static std::atomic<unsigned long long> done[64];
     int dev = 0;
@@ -246,14 +245,18 @@ int launch_attention(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
     }
     if (int rc = launch_after(kern, dim3(blocks), C::THREADS, C::SMEM_BYTES, st, tk, tv, a)) return rc;
     if (!join) return FP4ATTN_OK;
-    return launch_after(paged_join_kernel<OutT, D, NH>, dim3(blocks, a.heads_per_group), 128, 0, st, a);
+    return launch_after(paged_join_kernel<OutT, D, HC>, dim3(blocks, a.heads_per_group), 128, 0, st, a);
 }
 
 template <typename OutT, int D>
 int launch_heads(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
 {
-    return mma_heads(a.group) == 16 ? launch_attention<OutT, D, 16>(a, blocks, join, st)
-                                    : launch_attention<OutT, D, 32>(a, blocks, join, st);
+    switch (heads_at_once(a.group)) {
+        case 4: return launch_attention<OutT, D, 4>(a, blocks, join, st);
+        case 8: return launch_attention<OutT, D, 8>(a, blocks, join, st);
+        case 16: return launch_attention<OutT, D, 16>(a, blocks, join, st);
+        default: return launch_attention<OutT, D, 32>(a, blocks, join, st);
+    }
 }
 
 template <typename OutT>
@@ -473,7 +476,7 @@ int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out
     a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
     a.out = Out;
     a.lse = lse;
-    const int nh = mma_heads(a.group);
+    const int nh = heads_at_once(a.group);
     a.splits = (a.group + nh - 1) / nh;
     a.heads_per_group = (a.group + a.splits - 1) / a.splits;
     a.head_groups = cache->kv_heads * a.splits;

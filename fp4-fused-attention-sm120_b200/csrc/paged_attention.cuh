@@ -65,9 +65,15 @@ namespace fp4attn {
 constexpr int kPagedBlocks = 148;
 constexpr int kPagedTile = 128;
 
-template <int D, int NH, bool kSplitP>
+// HC: query heads computed (4, 8, 16 or 32, at least the group's share).
+template <int D, int HC, bool kSplitP>
 struct PagedCfg {
     static constexpr int THREADS = 384;
+    // Tiles a step: the roles wait for one another once a step.  Tiles of
+    // small heads are short, so two make a step.
+    static constexpr int U = D <= 64 ? 2 : 1;
+    static constexpr int NS = HC < 16 ? 16 : HC;                     // N of the S^T MMA
+    static constexpr int NP = kSplitP ? (2 * HC < 16 ? 16 : 2 * HC) : NS;  // N of the O^T MMA: with two parts, low parts from NP / 2 on
     static constexpr int KROW = D <= 64 ? 32 : D <= 128 ? 64 : 128;  // bytes of a key's codes in shared memory (= swizzle)
     static constexpr int KSTEPS = (D + 63) / 64;                     // mxf4 MMAs of K = 64 per S^T tile
     static constexpr int ATOMS = (KSTEPS + 1) / 2;                   // 512-byte scale atoms (four blocks of 32)
@@ -78,31 +84,30 @@ struct PagedCfg {
     static constexpr uint32_t VSW = CB == 128 ? ptx::kSwizzle128B : ptx::kSwizzle64B;
     static constexpr int DCH = D / CHE;
     static constexpr int MT = (D + 127) / 128;                       // O^T MMAs of M = 128 (rows past D are not read)
-    static constexpr int PARTS = kSplitP ? 2 : 1;
-    static constexpr int PROW = 2 * NH;                              // bytes of a key's P row (= swizzle)
-    static constexpr uint32_t PSW = PROW == 32 ? ptx::kSwizzle32B : ptx::kSwizzle64B;
+    static constexpr int PROW = 2 * NP;                              // bytes of a key's P row (= swizzle)
+    static constexpr uint32_t PSW = PROW == 32 ? ptx::kSwizzle32B : PROW == 64 ? ptx::kSwizzle64B : ptx::kSwizzle128B;
     // Tensor Memory columns
-    static constexpr int S_COL = 0;                                  // two buffers
-    static constexpr int O_COL = 2 * NH;                             // two buffers of MT
-    static constexpr int SFA_COL = O_COL + 2 * MT * NH;
+    static constexpr int S_COL = 0;                                  // [2][U][NS]
+    static constexpr int O_COL = 2 * U * NS;                         // [2][MT][NP]
+    static constexpr int SFA_COL = O_COL + 2 * MT * NP;
     static constexpr int SFB_COL = SFA_COL + 4 * ATOMS;
     static constexpr int TMEM_USED = SFB_COL + 4 * ATOMS;
-    static constexpr int TMEM_COLS = TMEM_USED <= 128 ? 128 : 256;
-    static_assert(TMEM_USED <= 256, "TMEM budget exceeded");
+    static constexpr int TMEM_COLS = TMEM_USED <= 128 ? 128 : TMEM_USED <= 256 ? 256 : 512;
+    static_assert(TMEM_USED <= 512, "TMEM budget exceeded");
     // shared memory, offsets from a 1024-aligned base
     static constexpr int align1k(int x) { return (x + 1023) / 1024 * 1024; }
     static constexpr int K_BYTES = kPagedTile * KROW;
     static constexpr int V_BYTES = kPagedTile * D * 2;
     static constexpr int S_BYTES = align1k(kPagedTile * NB);
     static constexpr int STAGE = K_BYTES + V_BYTES + S_BYTES;
-    static constexpr int OFF_P = 0;                                  // [2][PARTS][128 keys][PROW]
+    static constexpr int OFF_P = 0;                                  // [2][U][128 keys][PROW]
     static constexpr int P_BYTES = kPagedTile * PROW;
     static constexpr int QBUFS = 4;                                  // items whose queries may be ready ahead
-    static constexpr int OFF_Q = OFF_P + 2 * PARTS * P_BYTES;        // [QBUFS][NH rows][KROW]
-    static constexpr int Q_BYTES = align1k(NH * KROW);
+    static constexpr int OFF_Q = OFF_P + 2 * U * P_BYTES;            // [QBUFS][NS rows][KROW]
+    static constexpr int Q_BYTES = align1k(NS * KROW);
     static constexpr int OFF_QSF = OFF_Q + QBUFS * Q_BYTES;          // [QBUFS][ATOMS][512]
-    static constexpr int OFF_KSF = OFF_QSF + QBUFS * ATOMS * 512;    // [2][ATOMS][512]
-    static constexpr int OFF_STAGE = align1k(OFF_KSF + 2 * ATOMS * 512);
+    static constexpr int OFF_KSF = OFF_QSF + QBUFS * ATOMS * 512;    // [2][U][ATOMS][512]
+    static constexpr int OFF_STAGE = align1k(OFF_KSF + 2 * U * ATOMS * 512);
     // The O^T MMA reads 128 rows (head-dim columns) of V: past head_dim it
     // reads on into what follows; those rows of O^T are not used.
     static constexpr int V_OVER = (MT * 128 - D) / CHE * kPagedTile * CB;
@@ -117,8 +122,8 @@ struct PagedCfg {
 // The partial results of an item that spans blocks: slot 2 * block for a range
 // that began inside the item, 2 * block + 1 for the item begun in the range.
 struct PagedPartials {
-    float* o;        // [2 * kPagedBlocks][NH][D]
-    float2* ml;      // [2 * kPagedBlocks][NH]  maximum (log2 domain), sum
+    float* o;        // [2 * kPagedBlocks][HC][D]
+    float2* ml;      // [2 * kPagedBlocks][HC]  reference (log2 domain), sum
     int4* items;     // [kPagedBlocks]  sequence, head group, last block, first slot; sequence -1: none begun here goes on
 };
 
@@ -151,10 +156,17 @@ __device__ __forceinline__ int paged_length(const PagedArgs& a, int b)
 // Tiles of a sequence; an empty one has one (without keys), which writes its zeros.
 __device__ __forceinline__ int paged_tiles(int len) { return len <= 0 ? 1 : (len + kPagedTile - 1) / kPagedTile; }
 
-// First tile of a block's range out of `total`.
-__device__ __forceinline__ int paged_first(int64_t total, int block, int blocks)
+// First tile of a block's range, and the block whose range holds a tile:
+// `total` tiles dealt to `blocks` blocks (at most `total`), the first
+// total % blocks of which have one more.
+__device__ __forceinline__ int paged_first(int total, int block, int blocks)
 {
-    return static_cast<int>(total * block / blocks);
+    return block * (total / blocks) + min(block, total % blocks);
+}
+__device__ __forceinline__ int paged_block(int total, int tile, int blocks)
+{
+    const int base = total / blocks, more = total % blocks, head = more * (base + 1);
+    return tile < head ? tile / (base + 1) : more + (tile - head) / base;
 }
 
 // The walk over the items, or parts of items, in a block's range; every role
@@ -219,39 +231,30 @@ __device__ __forceinline__ void find_range(const PagedArgs& a, PagedRange* range
 {
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const bool scans = tid < 256;
-    int mine = 0, sum = 0;  // tiles of sequence tid; of sequences tid, tid + 256, ...
-    if (scans) {
-        if (tid < a.batch) mine = paged_tiles(paged_length(a, tid));
-        sum = mine;
-        for (int b = tid + 256; b < a.batch; b += 256) sum += paged_tiles(paged_length(a, b));
-        sum = __reduce_add_sync(~0u, sum);
-        if (lane == 0) scratch[warp] = sum;
-    }
-    __syncthreads();
-    int64_t total = 0;
+    // With up to 256 sequences one scan gives the total as well; with more, a
+    // sum over all of them comes first.
+    int sum = 0;
+    if (a.batch > 256) {
+        if (scans) {
+            for (int b = tid; b < a.batch; b += 256) sum += paged_tiles(paged_length(a, b));
+            sum = __reduce_add_sync(~0u, sum);
+            if (lane == 0) scratch[warp] = sum;
+        }
+        __syncthreads();
+        sum = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) total += scratch[i];
-    total *= a.head_groups;
-    const int blocks = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
-    const bool idle = static_cast<int>(blockIdx.x) >= blocks;
-    const int t0 = idle ? 0 : paged_first(total, blockIdx.x, blocks), t1 = idle ? 0 : paged_first(total, blockIdx.x + 1, blocks);
-    if (tid == 0) {
-        range->first = t0;
-        range->count = t1 - t0;
-        range->total = static_cast<int>(total);
-        range->blocks = blocks;
+        for (int i = 0; i < 8; i++) sum += scratch[i];
     }
-    if (idle) return;
     int carry = 0;  // tiles (of one head group) of the sequences before this chunk
     for (int b0 = 0; b0 < a.batch; b0 += 256) {
-        if (b0 > 0) mine = scans && b0 + tid < a.batch ? paged_tiles(paged_length(a, b0 + tid)) : 0;
+        const int mine = scans && b0 + tid < a.batch ? paged_tiles(paged_length(a, b0 + tid)) : 0;
         int inc = mine;
 #pragma unroll
         for (int i = 1; i < 32; i <<= 1) {
             const int v = __shfl_up_sync(~0u, inc, i);
             if (lane >= i) inc += v;
         }
-        __syncthreads();
+        if (a.batch > 256) __syncthreads();  // (the last chunk's sums have been read)
         if (scans && lane == 31) scratch[warp] = inc;
         __syncthreads();
         int before = carry, all = 0;
@@ -260,10 +263,20 @@ __device__ __forceinline__ void find_range(const PagedArgs& a, PagedRange* range
             if (i < warp) before += scratch[i];
             all += scratch[i];
         }
-        const int64_t at = static_cast<int64_t>(before + inc - mine) * a.head_groups;
-        if (scans && t0 >= at && t0 < at + static_cast<int64_t>(mine) * a.head_groups) {
-            const int in = static_cast<int>(t0 - at);
+        if (a.batch <= 256) sum = all;
+        const int total = sum * a.head_groups, blocks = min(total, static_cast<int>(gridDim.x));
+        const bool idle = static_cast<int>(blockIdx.x) >= blocks;
+        const int t0 = idle ? 0 : paged_first(total, blockIdx.x, blocks);
+        const int at = (before + inc - mine) * a.head_groups;
+        if (scans && !idle && t0 >= at && t0 < at + mine * a.head_groups) {
+            const int in = t0 - at;
             range->start = make_int4(b0 + tid, in / mine, in % mine, 0);
+        }
+        if (tid == 0) {
+            range->first = t0;
+            range->count = idle ? 0 : paged_first(total, blockIdx.x + 1, blocks) - t0;
+            range->total = total;
+            range->blocks = blocks;
         }
         carry += all;
     }
@@ -283,13 +296,13 @@ __device__ __forceinline__ float warp_reduce4(const float (&v)[4], int lane, Op 
     return op(k, __shfl_xor_sync(~0u, k, 1));
 }
 
-template <typename OutT, int D, int NH>
+template <typename OutT, int D, int HC>
 __global__ void __launch_bounds__(384, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                            const __grid_constant__ PagedArgs a)
 {
     constexpr bool kSplitP = sizeof(OutT) == 4;
-    using C = PagedCfg<D, NH, kSplitP>;
+    using C = PagedCfg<D, HC, kSplitP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_MISC);
@@ -298,13 +311,14 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t* empty = v_full + 8;          // [8] the stage's MMAs are done (commit)
     uint64_t* q_full = empty + 8;          // [4] query codes and scales written (32)
     uint64_t* q_empty = q_full + 4;        // [4] the item's S^T MMAs are done (commit)
+    // (these by step)
     uint64_t* s_full = q_empty + 4;        // [2][2] S^T computed (commit); by warpgroup, see below
     uint64_t* s_free = s_full + 4;         // [2] S^T in registers (128)
     uint64_t* p_full = s_free + 2;         // [2] P written (128)
     uint64_t* o_full = p_full + 2;         // [2] O^T computed, P read (commit)
     uint64_t* o_free = o_full + 2;         // [2] O^T in registers (128)
     uint64_t* drain = o_free + 2;          // [2] everything an issuer issued is done (exit)
-    float* red_all = reinterpret_cast<float*>(smem + C::OFF_MISC + 512);  // [2][4][NH]
+    float* red_all = reinterpret_cast<float*>(smem + C::OFF_MISC + 512);  // [2][4][HC]
     int* scratch = reinterpret_cast<int*>(smem + C::OFF_MISC + 1536);     // [8]
     PagedRange* range = reinterpret_cast<PagedRange*>(scratch + 8);
     uint32_t* tmem_sh = reinterpret_cast<uint32_t*>(scratch + 16);
@@ -464,59 +478,68 @@ __global__ void __launch_bounds__(384, 1)
         for (int wg = 0; ok && t.left > 0; t.next(a), qr.next(), wg ^= 1) {
             const int qb = qr.s;
             int j = own[wg];
-            own[wg] += t.n;
-            for (int i = 0; i < t.n; i++, g++, j++, ring.next()) {
+            const int n_steps = (t.n + C::U - 1) / C::U;
+            own[wg] += n_steps;
+            for (int i = 0; i < n_steps; i++, g++, j++) {
                 const int buf = g & 1;
-                // S^T and the scale atoms of tile g - 2 have been read.
+                // S^T and the scale atoms of step g - 2 have been read.
                 bool go = g < 2 || bounded_wait(&s_free[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedSFree);
-                go = bounded_wait(&k_full[ring.s], ring.parity, w, kPagedKFull) && go;
                 if (i == 0) go = bounded_wait(&q_full[qb], qr.parity, w, kPagedQFull) && go;
-                if (!__all_sync(~0u, go)) {
-                    ok = false;
-                    break;
-                }
-                // Lane l writes row l of each atom: the scales of keys l, 32 + l, 64 + l, 96 + l.
-                const uint8_t* raw = stages + ring.s * C::STAGE + C::K_BYTES + C::V_BYTES;
 #pragma unroll
-                for (int k = 0; k < C::ATOMS; k++) {
-                    uint32_t word[4];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint8_t* p = raw + (c * 32 + lane) * C::NB + 4 * k;
-                        if constexpr (C::NB % 4 == 0) {
-                            word[c] = *reinterpret_cast<const uint32_t*>(p);
-                        } else {
-                            word[c] = 0u;
-#pragma unroll
-                            for (int j = 0; j < 4; j++) word[c] |= (4 * k + j < C::NB ? p[j] : 127u) << (8 * j);
-                        }
+                for (int u = 0; u < C::U; u++) {
+                    if (u > 0 && i * C::U + u >= t.n) break;
+                    go = bounded_wait(&k_full[ring.s], ring.parity, w, kPagedKFull) && go;
+                    if (!__all_sync(~0u, go)) {
+                        ok = false;
+                        break;
                     }
-                    *reinterpret_cast<uint4*>(smem + C::OFF_KSF + (buf * C::ATOMS + k) * 512 + lane * 16) =
-                        make_uint4(word[0], word[1], word[2], word[3]);
-                }
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    ptx::tc_fence_after();
-                    if (i == 0)
+                    // Lane l writes row l of each atom: the scales of keys l, 32 + l, 64 + l, 96 + l.
+                    const uint8_t* raw = stages + ring.s * C::STAGE + C::K_BYTES + C::V_BYTES;
+#pragma unroll
+                    for (int k = 0; k < C::ATOMS; k++) {
+                        uint32_t word[4];
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const uint8_t* p = raw + (c * 32 + lane) * C::NB + 4 * k;
+                            if constexpr (C::NB % 4 == 0) {
+                                word[c] = *reinterpret_cast<const uint32_t*>(p);
+                            } else {
+                                word[c] = 0u;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) word[c] |= (4 * k + e < C::NB ? p[e] : 127u) << (8 * e);
+                            }
+                        }
+                        *reinterpret_cast<uint4*>(smem + C::OFF_KSF + ((buf * C::U + u) * C::ATOMS + k) * 512 + lane * 16) =
+                            make_uint4(word[0], word[1], word[2], word[3]);
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::tc_fence_after();
+                        if (i == 0 && u == 0)
+#pragma unroll
+                            for (int k = 0; k < C::ATOMS; k++)
+                                ptx::tc_cp_32x128b_warpx4(tmem + C::SFB_COL + 4 * k, sfb0 + (qb * C::ATOMS + k) * (512 / 16));
 #pragma unroll
                         for (int k = 0; k < C::ATOMS; k++)
-                            ptx::tc_cp_32x128b_warpx4(tmem + C::SFB_COL + 4 * k, sfb0 + (qb * C::ATOMS + k) * (512 / 16));
+                            ptx::tc_cp_32x128b_warpx4(tmem + C::SFA_COL + 4 * k, sfa0 + ((buf * C::U + u) * C::ATOMS + k) * (512 / 16));
+                        const uint64_t kd = kd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16)), qd = qd0 + qb * (C::Q_BYTES / 16);
 #pragma unroll
-                    for (int k = 0; k < C::ATOMS; k++)
-                        ptx::tc_cp_32x128b_warpx4(tmem + C::SFA_COL + 4 * k, sfa0 + (buf * C::ATOMS + k) * (512 / 16));
-                    const uint64_t kd = kd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16)), qd = qd0 + qb * (C::Q_BYTES / 16);
-#pragma unroll
-                    for (int kk = 0; kk < C::KSTEPS; kk++) {
-                        const uint32_t id = 2u * (kk & 1);
-                        ptx::mma_mxf4(tmem + C::S_COL + buf * NH, kd + 2 * kk, qd + 2 * kk, ptx::idesc_mxf4(128, NH, id, id),
-                                      (tmem + C::SFA_COL + 4 * (kk / 2)) | (id << 30),
-                                      (tmem + C::SFB_COL + 4 * (kk / 2)) | (id << 30), kk > 0 ? 1u : 0u);
+                        for (int kk = 0; kk < C::KSTEPS; kk++) {
+                            const uint32_t id = 2u * (kk & 1);
+                            ptx::mma_mxf4(tmem + C::S_COL + (buf * C::U + u) * C::NS, kd + 2 * kk, qd + 2 * kk,
+                                          ptx::idesc_mxf4(128, C::NS, id, id), (tmem + C::SFA_COL + 4 * (kk / 2)) | (id << 30),
+                                          (tmem + C::SFB_COL + 4 * (kk / 2)) | (id << 30), kk > 0 ? 1u : 0u);
+                        }
                     }
-                    ptx::tc_commit(&s_full[2 * wg + (j & 1)]);
-                    if (i + 1 == t.n) ptx::tc_commit(&q_empty[qb]);
+                    __syncwarp();
+                    ring.next();
                 }
-                __syncwarp();
+                if (!ok) break;
+                if (lane == 0) {
+                    ptx::tc_commit(&s_full[2 * wg + (j & 1)]);
+                    if (i + 1 == n_steps) ptx::tc_commit(&q_empty[qb]);
+                }
             }
         }
         if (lane == 0) {  // everything issued completes before Tensor Memory is freed
@@ -527,43 +550,56 @@ __global__ void __launch_bounds__(384, 1)
     } else if (warp == 3) {
         // ------------------------------------------------------------ O^T issuer
         if (lane == 0) {
-            constexpr uint32_t idesc_o = ptx::idesc_f16x(128, NH, 0, true, true);
-            // V's 16-key steps within a stage (in 16-byte units): page by page, rows within a page.
-            uint64_t vo[8];
+            constexpr uint32_t idesc_o = ptx::idesc_f16x(128, C::NP, 0, true, true);
+            // V's 16-key steps within a stage, in 16-byte units: page by page, rows within a page.
+            auto v_at = [&](int kk) {
+                return static_cast<uint32_t>((((kk * 16) >> shift) * page * D * 2 + ((kk * 16) & (page - 1)) * C::CB) >> 4);
+            };
+            uint32_t vo[8];
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++)
-                vo[kk] = static_cast<uint64_t>((((kk * 16) >> shift) * page * D * 2 + ((kk * 16) & (page - 1)) * C::CB) >> 4);
+            for (int kk = 0; kk < 8; kk++) vo[kk] = v_at(kk);
             const uint64_t vd0 = ptx::make_sdesc(ptx::smem_u32(stages + C::K_BYTES), page * C::CB, 8 * C::CB, C::VSW);
             const uint64_t pd0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_P), C::P_BYTES, 8 * C::PROW, C::PSW);
-            const uint64_t m_step = static_cast<uint64_t>((128 / C::CHE) * page * C::CB / 16);
+            const uint32_t m_step = static_cast<uint32_t>((128 / C::CHE) * page * C::CB / 16);
             Ring<C::STAGES> ring;
             int g = 0;
             bool ok = true;
             for (; ok && t.left > 0; t.next(a)) {
-                for (int i = 0; i < t.n; i++, g++, ring.next()) {
+                const int n_steps = (t.n + C::U - 1) / C::U;
+                for (int i = 0; ok && i < n_steps; i++, g++) {
                     const int buf = g & 1;
-                    const int steps = max(1, (t.keys(i) + 15) / 16);
-                    const uint64_t vd = vd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16));
-                    const uint64_t pd = pd0 + static_cast<uint64_t>(buf * C::PARTS * C::P_BYTES / 16);
-                    const uint32_t od = tmem + C::O_COL + buf * C::MT * NH;
                     ok = (g < 2 || bounded_wait(&o_free[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedOFree)) &&
-                         bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull) &&
                          bounded_wait(&p_full[buf], static_cast<uint32_t>(g / 2) & 1u, w, kPagedPFull);
-                    if (!ok) break;
-                    ptx::tc_fence_after();
 #pragma unroll
-                    for (int kk = 0; kk < 8; kk++) {
-                        if (kk >= steps) break;
+                    for (int u = 0; u < C::U; u++) {
+                        const int ti = i * C::U + u;
+                        if (u > 0 && ti >= t.n) break;
+                        ok = ok && bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+                        const uint64_t vd = vd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16));
+                        const uint64_t pd = pd0 + static_cast<uint64_t>((buf * C::U + u) * C::P_BYTES / 16);
+                        const uint32_t od = tmem + C::O_COL + buf * C::MT * C::NP;
+                        const int keys = t.keys(ti);
+                        if (keys > kPagedTile - 16) {
 #pragma unroll
-                        for (int part = 0; part < C::PARTS; part++)
+                            for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-                            for (int m = 0; m < C::MT; m++)
-                                ptx::mma_f16_ss(od + m * NH, vd + vo[kk] + m * m_step,
-                                                pd + (part * C::P_BYTES + kk * 16 * C::PROW) / 16, idesc_o,
-                                                (kk > 0 || part > 0) ? 1u : 0u);
+                                for (int m = 0; m < C::MT; m++)
+                                    ptx::mma_f16_ss(od + m * C::NP, vd + (vo[kk] + m * m_step), pd + kk * C::PROW, idesc_o,
+                                                    (kk > 0 || u > 0) ? 1u : 0u);
+                        } else {
+#pragma unroll 1
+                            for (int kk = 0; kk < max(1, (keys + 15) / 16); kk++)
+#pragma unroll
+                                for (int m = 0; m < C::MT; m++)
+                                    ptx::mma_f16_ss(od + m * C::NP, vd + (v_at(kk) + m * m_step), pd + kk * C::PROW, idesc_o,
+                                                    (kk > 0 || u > 0) ? 1u : 0u);
+                        }
+                        ptx::tc_commit(&empty[ring.s]);
+                        ring.next();
                     }
-                    ptx::tc_commit(&o_full[buf]);
-                    ptx::tc_commit(&empty[ring.s]);
+                    if (ok) ptx::tc_commit(&o_full[buf]);
                 }
             }
             ptx::tc_commit(&drain[1]);
@@ -575,228 +611,209 @@ __global__ void __launch_bounds__(384, 1)
         const int wg = (warp - 4) / 4, wq = warp % 4, row = wq * 32 + lane;  // key of the tile; head-dim row of O^T
         const uint32_t lanes = tmem + (static_cast<uint32_t>(wq * 32) << 16);
         const int bar_id = 1 + wg;
-        float* red = red_all + wg * 4 * NH;
+        float* red = red_all + wg * 4 * HC;
         constexpr float kGrowth = 8.f;  // how far (log2) a score may exceed the reference
-        constexpr int CH = NH / 4;      // heads in fours: fours past the group's heads are skipped
-        float nm[NH], l[NH], o[C::MT][NH];  // minus the reference, this thread's sums, O^T
+        float nm[HC], l[HC], o[C::MT][HC];  // minus the reference, this thread's sums, O^T
         bool ok = true;  // no wait of this thread has run out
-        auto load_cols = [&](uint32_t col, uint32_t (&r)[NH]) {
-            if constexpr (NH == 16) ptx::tmem_ld16(lanes + col, r);
+        auto load_cols = [&](uint32_t col, uint32_t (&r)[HC]) {
+            if constexpr (HC == 4) ptx::tmem_ld4(lanes + col, r);
+            else if constexpr (HC == 8) ptx::tmem_ld8(lanes + col, r);
+            else if constexpr (HC == 16) ptx::tmem_ld16(lanes + col, r);
             else ptx::tmem_ld32(lanes + col, r);
         };
         auto max_of = [](float x, float y) { return fmaxf(x, y); };
         auto sum_of = [](float x, float y) { return x + y; };
         Ring<C::STAGES> ring;
-        int g = 0, j = 0;  // tile of the block, tile of this warpgroup
+        int g = 0, j = 0;  // step of the block, step of this warpgroup
         for (int item = 0; t.left > 0; t.next(a), item++) {
+            const int n_steps = (t.n + C::U - 1) / C::U;
             if ((item & 1) != wg) {  // the other warpgroup's
-                g += t.n;
+                g += n_steps;
                 for (int i = t.n % C::STAGES; i > 0; i--) ring.next();
                 ring.parity ^= static_cast<uint32_t>(t.n / C::STAGES) & 1u;
                 continue;
             }
-            const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
-            // Adds tile g's O^T to the registers.
-            auto add_o = [&](int tile_g) {
-                const int buf = tile_g & 1;
-                if (!__all_sync(~0u, bounded_wait(&o_full[buf], static_cast<uint32_t>(tile_g / 2) & 1u, w, kPagedOFull))) {
-                    ok = false;
-                    return;
-                }
-                ptx::tc_fence_after();
-                uint32_t r[C::MT][NH];
+            bool out_of_time = false;
+            // Step i: P, then the O^T of step i - 1 is added (the last has no P).
+            for (int i = 0; i <= n_steps; i++) {
+                float beta[HC];  // what moves step i - 1's O^T to the present reference
 #pragma unroll
-                for (int m = 0; m < C::MT; m++) load_cols(C::O_COL + (buf * C::MT + m) * NH, r[m]);
-                ptx::tc_wait_ld();
-                ptx::tc_fence_before();
-                ptx::mbar_arrive(&o_free[buf]);
+                for (int h = 0; h < HC; h++) beta[h] = 1.f;
+                if (i < n_steps) {
+                    const int buf = g & 1;
+                    ok = bounded_wait(&s_full[2 * wg + (j & 1)], static_cast<uint32_t>(j / 2) & 1u, w, kPagedSFull) && ok;
+                    __syncwarp();
+                    ptx::tc_fence_after();
+                    uint32_t sr[C::U][HC];
 #pragma unroll
-                for (int c = 0; c < CH; c++)
-                    if (4 * c < nh)
+                    for (int u = 0; u < C::U; u++) load_cols(C::S_COL + (buf * C::U + u) * C::NS, sr[u]);
+                    ptx::tc_wait_ld();
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(&s_free[buf]);
+                    float x[C::U][HC];  // the scores, log2 domain, less the reference
+                    bool over = i == 0 || !ok;
 #pragma unroll
-                        for (int m = 0; m < C::MT; m++)
+                    for (int u = 0; u < C::U; u++) {
+                        const int keys = i * C::U + u < t.n ? t.keys(i * C::U + u) : 0;
+                        if (row >= keys)
 #pragma unroll
-                            for (int h = 4 * c; h < 4 * c + 4; h++) o[m][h] += __uint_as_float(r[m][h]);
-            };
-            bool pending = false, out_of_time = false;  // pending: tile g - 1's O^T is not yet added
-            for (int i = 0; i < t.n; i++, g++, j++, ring.next()) {
-                const int buf = g & 1, n = t.keys(i);
-                ok = __all_sync(~0u, bounded_wait(&s_full[2 * wg + (j & 1)], static_cast<uint32_t>(j / 2) & 1u, w, kPagedSFull)) && ok;
-                ptx::tc_fence_after();
-                uint32_t sr[NH];
-                load_cols(C::S_COL + buf * NH, sr);
-                ptx::tc_wait_ld();
-                ptx::tc_fence_before();
-                ptx::mbar_arrive(&s_free[buf]);
-                float x[NH];  // the scores, log2 domain, less the reference
-                bool over = i == 0 || !ok;
-                if (n < kPagedTile)
+                            for (int h = 0; h < HC; h++) sr[u][h] = 0xFF800000u;  // -inf
 #pragma unroll
-                    for (int h = 0; h < NH; h++)
-                        if (row >= n) sr[h] = 0xFF800000u;  // -inf
-                if (i == 0) {
-#pragma unroll
-                    for (int h = 0; h < NH; h++) nm[h] = 0.f;
-                }
-#pragma unroll
-                for (int c = 0; c < CH; c++)
-                    if (4 * c < nh)
-#pragma unroll
-                        for (int h = 4 * c; h < 4 * c + 4; h++) {
-                            x[h] = fmaf(__uint_as_float(sr[h]), a.scale_log2, nm[h]);
-                            over |= x[h] > kGrowth;
+                        for (int h = 0; h < HC; h++) {
+                            if (i == 0) nm[h] = 0.f;
+                            x[u][h] = fmaf(__uint_as_float(sr[u][h]), a.scale_log2, nm[h]);
+                            over |= x[u][h] > kGrowth;
                         }
-                if (ptx::named_bar_any(bar_id, 128, over)) {
-                    // Rare: a new item, a score that outgrew the reference, or
-                    // a wait that ran out.  All 128 threads come here together.
-                    if (ptx::named_bar_any(bar_id, 128, !ok)) {
-                        out_of_time = true;
-                        break;
                     }
-                    if (pending) {
-                        add_o(g - 1);
-                        pending = false;
-                    }
+                    if (ptx::named_bar_any(bar_id, 128, over)) {
+                        // Rare: a new item, a score that outgrew the reference, or
+                        // a wait that ran out.  All 128 threads come here together.
+                        if (ptx::named_bar_any(bar_id, 128, !ok)) {
+                            out_of_time = true;
+                            break;
+                        }
 #pragma unroll
-                    for (int c = 0; c < CH; c++)
-                        if (4 * c < nh) {
-                            const float v[4] = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+                        for (int c = 0; c < HC / 4; c++) {
+                            float v[4];
+#pragma unroll
+                            for (int q = 0; q < 4; q++) v[q] = C::U == 2 ? fmaxf(x[0][4 * c + q], x[C::U - 1][4 * c + q]) : x[0][4 * c + q];
                             const float top = warp_reduce4(v, lane, max_of);
-                            if ((lane & 7) == 0) red[wq * NH + 4 * c + (lane >> 3)] = top;
+                            if ((lane & 7) == 0) red[wq * HC + 4 * c + (lane >> 3)] = top;
                         }
-                    ptx::named_bar_sync(bar_id, 128);
+                        ptx::named_bar_sync(bar_id, 128);
 #pragma unroll
-                    for (int c = 0; c < CH; c++)
-                        if (4 * c < nh) {
-                            float top[4];
+                        for (int h = 0; h < HC; h++) {
+                            const float top = fmaxf(fmaxf(red[h], red[HC + h]), fmaxf(red[2 * HC + h], red[3 * HC + h]));
+                            // How far the reference moves: up, or at an item's start to the
+                            // maximum (0 when there is no key at all).
+                            const float up = i > 0 ? fmaxf(top, 0.f) : top == -INFINITY ? 0.f : top;
+                            beta[h] = i > 0 ? ptx::ex2_approx(-up) : 0.f;
+                            nm[h] -= up;
 #pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const float4 f = *reinterpret_cast<const float4*>(red + q * NH + 4 * c);
-                                top[0] = q ? fmaxf(top[0], f.x) : f.x;
-                                top[1] = q ? fmaxf(top[1], f.y) : f.y;
-                                top[2] = q ? fmaxf(top[2], f.z) : f.z;
-                                top[3] = q ? fmaxf(top[3], f.w) : f.w;
-                            }
+                            for (int u = 0; u < C::U; u++) x[u][h] -= up;
+                            l[h] = i > 0 ? l[h] * beta[h] : 0.f;
 #pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                // How far the reference moves: up, or at an item's start to the maximum (0
-                                // when there is no key at all).
-                                const int h = 4 * c + q;
-                                const float up = i > 0 ? fmaxf(top[q], 0.f) : top[q] == -INFINITY ? 0.f : top[q];
-                                const float alpha = i > 0 ? ptx::ex2_approx(-up) : 0.f;
-                                nm[h] -= up;
-                                x[h] -= up;
-                                l[h] = i > 0 ? l[h] * alpha : 0.f;
+                            for (int m = 0; m < C::MT; m++) o[m][h] = i > 0 ? o[m][h] * beta[h] : 0.f;
+                        }
+                    }
+                    // P of these keys.  Its buffer was last read by step g - 2's O^T:
+                    // added already, unless the other warpgroup had it.  (Step g - 4's
+                    // is complete then, so the parity is unambiguous: if it was the
+                    // other warpgroup's, that added it before it read S^T of g - 2.)
+                    if (i < 2 && g >= 2)
+                        ok = bounded_wait(&o_full[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedOFull) && ok;
 #pragma unroll
-                                for (int m = 0; m < C::MT; m++) o[m][h] = i > 0 ? o[m][h] * alpha : 0.f;
+                    for (int u = 0; u < C::U; u++) {
+                        if (u > 0 && i * C::U + u >= t.n) break;
+                        uint32_t hi[HC / 2], lo[HC / 2];
+#pragma unroll
+                        for (int h = 0; h < HC; h += 2) {
+                            const float p0 = ptx::ex2_approx(x[u][h]), p1 = ptx::ex2_approx(x[u][h + 1]);
+                            l[h] += p0;
+                            l[h + 1] += p1;
+                            hi[h / 2] = ptx::pack_half2(p0, p1);
+                            if constexpr (kSplitP) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[h / 2]));
+                                lo[h / 2] = ptx::pack_half2(p0 - f.x, p1 - f.y);
                             }
                         }
-                }
-                // P of this key.  Its buffer was last read by tile g - 2's O^T:
-                // added above, unless the other warpgroup had it.  (Tile g - 4's
-                // is complete then, so the parity is unambiguous: if it was the
-                // other warpgroup's, that added it before it read S^T of g - 2.)
-                if (i < 2 && g >= 2)
-                    ok = __all_sync(~0u, bounded_wait(&o_full[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedOFull)) && ok;
-                uint8_t* p = smem + C::OFF_P + buf * C::PARTS * C::P_BYTES + row * C::PROW;
-                const int sw = C::PROW == 32 ? (row >> 2) & 1 : (row >> 1) & 3;
+                        uint8_t* p = smem + C::OFF_P + (buf * C::U + u) * C::P_BYTES + row * C::PROW;
+                        const int sw = C::PROW == 32 ? (row >> 2) & 1 : C::PROW == 64 ? (row >> 1) & 3 : row & 7;
+                        auto put = [&](int column, const uint32_t (&v)[HC / 2]) {  // HC columns from `column` on
+                            if constexpr (HC == 4) {
+                                *reinterpret_cast<uint2*>(p + (((column / 8) ^ sw) * 16)) = make_uint2(v[0], v[1]);
+                            } else {
 #pragma unroll
-                for (int u = 0; u < NH / 8; u++) {
-                    if (8 * u >= nh) break;
-                    uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-                    for (int c = 2 * u; c < 2 * u + 2; c++)
-                        if (4 * c < nh)
-#pragma unroll
-                            for (int h = 4 * c; h < 4 * c + 4; h += 2) {
-                                const float p0 = ptx::ex2_approx(x[h]), p1 = ptx::ex2_approx(x[h + 1]);
-                                l[h] += p0;
-                                l[h + 1] += p1;
-                                const uint32_t pk = ptx::pack_half2(p0, p1);
-                                hi[(h - 8 * u) / 2] = pk;
-                                if constexpr (kSplitP) {
-                                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pk));
-                                    lo[(h - 8 * u) / 2] = ptx::pack_half2(p0 - f.x, p1 - f.y);
-                                }
+                                for (int c = 0; c < HC / 8; c++)
+                                    *reinterpret_cast<uint4*>(p + (((column / 8 + c) ^ sw) * 16)) =
+                                        make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
                             }
-                    *reinterpret_cast<uint4*>(p + ((u ^ sw) * 16)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (kSplitP)
-                        *reinterpret_cast<uint4*>(p + C::P_BYTES + ((u ^ sw) * 16)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        };
+                        put(0, hi);
+                        if constexpr (kSplitP) put(C::NP / 2, lo);
+                        const int keys = t.keys(i * C::U + u);
+                        if (keys < kPagedTile) {
+                            if (row >= keys && row < max(16, (keys + 15) / 16 * 16)) {
+                                // A key behind the last: whatever lies in its place of V
+                                // (NaN included) must not meet its weight of zero.
+                                ok = bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull) && ok;
+                                uint8_t* v = stages + ring.s * C::STAGE + C::K_BYTES + (row >> shift) * page * D * 2 + (row & (page - 1)) * C::CB;
+#pragma unroll 1
+                                for (int c = 0; c < C::DCH * (C::CB / 16); c++)
+                                    *reinterpret_cast<uint4*>(v + c / (C::CB / 16) * page * C::CB + c % (C::CB / 16) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            }
+                        }
+                        ring.next();
+                    }
+                    __syncwarp();
+                    ptx::fence_proxy_async_smem();
+                    ptx::mbar_arrive(&p_full[buf]);
+                    g++;
+                    j++;
                 }
-                if (row >= n && row < max(16, (n + 15) / 16 * 16)) {
-                    // A key behind the last: whatever lies in its place of V
-                    // (NaN included) must not meet its weight of zero.
-                    ok = bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull) && ok;
-                    uint8_t* v = stages + ring.s * C::STAGE + C::K_BYTES + (row >> shift) * page * D * 2 + (row & (page - 1)) * C::CB;
-                    for (int c = 0; c < C::DCH; c++)
+                if (i > 0) {
+                    const int done = g - (i < n_steps ? 2 : 1), buf = done & 1;  // step i - 1
+                    ok = bounded_wait(&o_full[buf], static_cast<uint32_t>(done / 2) & 1u, w, kPagedOFull) && ok;
+                    __syncwarp();
+                    ptx::tc_fence_after();
+                    uint32_t r[C::MT][HC], r2[C::MT][HC];
 #pragma unroll
-                        for (int u = 0; u < C::CB / 16; u++)
-                            *reinterpret_cast<uint4*>(v + c * page * C::CB + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    for (int m = 0; m < C::MT; m++) {
+                        load_cols(C::O_COL + (buf * C::MT + m) * C::NP, r[m]);
+                        if constexpr (kSplitP) load_cols(C::O_COL + (buf * C::MT + m) * C::NP + C::NP / 2, r2[m]);
+                    }
+                    ptx::tc_wait_ld();
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(&o_free[buf]);
+#pragma unroll
+                    for (int m = 0; m < C::MT; m++)
+#pragma unroll
+                        for (int h = 0; h < HC; h++) {
+                            float v = __uint_as_float(r[m][h]);
+                            if constexpr (kSplitP) v += __uint_as_float(r2[m][h]);
+                            o[m][h] = fmaf(v, beta[h], o[m][h]);
+                        }
                 }
-                __syncwarp();
-                ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive(&p_full[buf]);
-                if (pending) add_o(g - 1);
-                pending = true;
             }
             if (out_of_time) break;
-            // The item's end in this block: g is one past its last tile here.
+            // The item's end in this block.
 #pragma unroll
-            for (int c = 0; c < CH; c++)
-                if (4 * c < nh) {
-                    const float v[4] = {l[4 * c], l[4 * c + 1], l[4 * c + 2], l[4 * c + 3]};
-                    const float sum = warp_reduce4(v, lane, sum_of);
-                    if ((lane & 7) == 0) red[wq * NH + 4 * c + (lane >> 3)] = sum;
-                }
+            for (int c = 0; c < HC / 4; c++) {
+                const float v[4] = {l[4 * c], l[4 * c + 1], l[4 * c + 2], l[4 * c + 3]};
+                const float sum = warp_reduce4(v, lane, sum_of);
+                if ((lane & 7) == 0) red[wq * HC + 4 * c + (lane >> 3)] = sum;
+            }
             ptx::named_bar_sync(bar_id, 128);
-            add_o(g - 1);
+            const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
             const bool begun = t.tile == 0;  // the item's first tile is in the range
             const bool whole = begun && t.n == t.tiles;
             const int slot = 2 * blockIdx.x + (t.left < count ? 1 : 0);
             const int64_t o0 = static_cast<int64_t>(t.b) * a.q_heads + (t.hg / a.splits) * a.group + h0;
 #pragma unroll
-            for (int c = 0; c < CH; c++) {
-                if (4 * c >= nh) break;
-                float sum[4];
+            for (int h = 0; h < HC; h++) {
+                if (h >= nh) break;
+                const float sum = (red[h] + red[HC + h]) + (red[2 * HC + h] + red[3 * HC + h]);
+                if (whole) {
+                    const float inv = sum > 0.f ? __fdividef(1.0f, sum) : 0.f;
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const float4 f = *reinterpret_cast<const float4*>(red + q * NH + 4 * c);
-                    sum[0] = q ? sum[0] + f.x : f.x;
-                    sum[1] = q ? sum[1] + f.y : f.y;
-                    sum[2] = q ? sum[2] + f.z : f.z;
-                    sum[3] = q ? sum[3] + f.w : f.w;
-                }
+                    for (int m = 0; m < C::MT; m++)
+                        if (m * 128 + row < D)
+                            static_cast<OutT*>(a.out)[(o0 + h) * D + m * 128 + row] = from_float<OutT>(o[m][h] * inv);
+                    if (a.lse && row == h)
+                        a.lse[o0 + h] = sum > 0.f ? (__log2f(sum) - nm[h]) * 0.6931471805599453f : INFINITY;
+                } else {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int h = 4 * c + q;
-                    if (h >= nh) break;
-                    if (whole) {
-                        const float inv = sum[q] > 0.f ? 1.0f / sum[q] : 0.f;
-#pragma unroll
-                        for (int m = 0; m < C::MT; m++)
-                            if (m * 128 + row < D)
-                                static_cast<OutT*>(a.out)[(o0 + h) * D + m * 128 + row] = from_float<OutT>(o[m][h] * inv);
-                        if (a.lse && row == h)
-                            a.lse[o0 + h] = sum[q] > 0.f ? (log2f(sum[q]) - nm[h]) * 0.6931471805599453f : INFINITY;
-                    } else {
-#pragma unroll
-                        for (int m = 0; m < C::MT; m++)
-                            if (m * 128 + row < D)
-                                a.p.o[(static_cast<int64_t>(slot) * NH + h) * D + m * 128 + row] = o[m][h];
-                        if (row == h) a.p.ml[slot * NH + h] = make_float2(-nm[h], sum[q]);
-                    }
+                    for (int m = 0; m < C::MT; m++)
+                        if (m * 128 + row < D)
+                            a.p.o[(static_cast<int64_t>(slot) * HC + h) * D + m * 128 + row] = o[m][h];
+                    if (row == h) a.p.ml[slot * HC + h] = make_float2(-nm[h], sum);
                 }
             }
             if (row == 0 && t.left == t.n) {
                 // What the join has to do for this block: the item begun here that goes on.
                 int4 it = make_int4(-1, 0, 0, 0);
-                if (begun && !whole) {
-                    const int64_t total = range->total, last = range->first + count - t.n + t.tiles - 1;  // its last tile
-                    int c = static_cast<int>(last * range->blocks / total);
-                    while (c + 1 < range->blocks && paged_first(total, c + 1, range->blocks) <= last) c++;
-                    while (paged_first(total, c, range->blocks) > last) c--;
-                    it = make_int4(t.b, t.hg, c, slot);
-                }
+                if (begun && !whole)  // (to the block of its last tile)
+                    it = make_int4(t.b, t.hg, paged_block(range->total, range->first + count - t.n + t.tiles - 1, range->blocks), slot);
                 a.p.items[blockIdx.x] = it;
             }
             ptx::named_bar_sync(bar_id, 128);  // (red is free again)
@@ -814,7 +831,7 @@ __global__ void __launch_bounds__(384, 1)
 
 // Block (j, h): head h of the item that attention block j began and others
 // continued: their partial results, in the blocks' order.
-template <typename OutT, int D, int NH>
+template <typename OutT, int D, int HC>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a)
 {
     ptx::grid_dependency_wait();
@@ -828,14 +845,14 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     const int parts = it.z - blockIdx.x + 1;
     auto slot = [&](int p) { return p == 0 ? it.w : 2 * (static_cast<int>(blockIdx.x) + p); };
     float top = -INFINITY;
-    for (int p = tid; p < parts; p += 128) top = fmaxf(top, a.p.ml[slot(p) * NH + h].x);
+    for (int p = tid; p < parts; p += 128) top = fmaxf(top, a.p.ml[slot(p) * HC + h].x);
     top = ptx::warp_max(top);
     if (tid % 32 == 0) red[tid / 32] = top;
     __syncthreads();
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float sum = 0.f;
     for (int p = tid; p < parts; p += 128) {
-        const float2 ml = a.p.ml[slot(p) * NH + h];
+        const float2 ml = a.p.ml[slot(p) * HC + h];
         const float wgt = ptx::ex2_approx(ml.x - top);
         weight[p] = wgt;
         sum += wgt * ml.y;
@@ -848,7 +865,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     for (int d = tid; d < D; d += 128) {
         float o = 0.f;
 #pragma unroll 4
-        for (int p = 0; p < parts; p++) o = fmaf(weight[p], a.p.o[(static_cast<int64_t>(slot(p)) * NH + h) * D + d], o);
+        for (int p = 0; p < parts; p++) o = fmaf(weight[p], a.p.o[(static_cast<int64_t>(slot(p)) * HC + h) * D + d], o);
         static_cast<OutT*>(a.out)[at * D + d] = from_float<OutT>(o / sum);
     }
     if (a.lse && tid == 0) a.lse[at] = (top + log2f(sum)) * 0.6931471805599453f;
