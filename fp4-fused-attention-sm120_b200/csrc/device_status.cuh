@@ -61,24 +61,32 @@ struct ServingWait {
     unsigned long long timeout_ns;
 };
 
-__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, const ServingWait& w, int site)
+// The part of a wait that runs when the phase is not complete at first sight,
+// out of line: a role's loop has several waits, and the roles of a block share
+// the SM's small instruction cache.
+static __device__ __noinline__ bool bounded_wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                    unsigned long long timeout_ns, int site)
 {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = ptx::globaltimer_ns();
     for (uint32_t it = 1; it < (1u << 30); ++it) {
         if (ptx::mbar_try_wait(bar, parity)) return true;
         if ((it & 31u) == 0u) {
-            if (*w.abort_flag) return false;
-            if (ptx::globaltimer_ns() - t0 > w.timeout_ns) break;
+            if (*abort_flag) return false;
+            if (ptx::globaltimer_ns() - t0 > timeout_ns) break;
         }
     }
-    *w.abort_flag = 1;
+    *abort_flag = 1;
     record_serving_timeout(site);
     return false;
 }
 
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, const ServingWait& w, int site)
+{
+    return ptx::mbar_try_wait(bar, parity) || bounded_wait_on(bar, parity, w.abort_flag, w.timeout_ns, site);
+}
+
 // On the way out: waits for what is in flight whatever the abort flag says.
-__device__ __forceinline__ void bounded_drain(uint64_t* bar, uint32_t parity, unsigned long long ns)
+static __device__ __noinline__ void bounded_drain(uint64_t* bar, uint32_t parity, unsigned long long ns)
 {
     const uint64_t t0 = ptx::globaltimer_ns();
     for (uint32_t it = 0; it < (1u << 30); ++it) {

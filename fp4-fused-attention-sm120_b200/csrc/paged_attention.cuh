@@ -296,6 +296,15 @@ __device__ __forceinline__ float warp_reduce4(const float (&v)[4], int lane, Op 
     return op(k, __shfl_xor_sync(~0u, k, 1));
 }
 
+// One block of 32 of a query row, quantised; out of line, for it is long and
+// runs once an item.
+static __device__ __noinline__ uint32_t quantize_query(const void* q, int64_t at, int half, int ocp, uint4* packed)
+{
+    const uint32_t sb = half ? quantize32<__half>(static_cast<const __half*>(q) + at, ocp, *packed)
+                             : quantize32<float>(static_cast<const float*>(q) + at, ocp, *packed);
+    return sb == 255u ? 254u : sb;
+}
+
 template <typename OutT, int D, int HC>
 __global__ void __launch_bounds__(384, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -443,9 +452,7 @@ __global__ void __launch_bounds__(384, 1)
                     const int r = k / C::NB, blk = k % C::NB;
                     const int64_t at = q0 + r * a.qh + blk * 32;
                     uint4 packed;
-                    uint32_t sb = a.q_half ? quantize32<__half>(static_cast<const __half*>(a.q) + at, a.ocp, packed)
-                                           : quantize32<float>(static_cast<const float*>(a.q) + at, a.ocp, packed);
-                    if (sb == 255u) sb = 254u;
+                    const uint32_t sb = quantize_query(a.q, at, a.q_half, a.ocp, &packed);
                     const int sw = C::KROW == 32 ? (r >> 2) & 1 : C::KROW == 64 ? (r >> 1) & 3 : r & 7;
                     *reinterpret_cast<uint4*>(smem + C::OFF_Q + qr.s * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16)) = packed;
                     smem[C::OFF_QSF + (qr.s * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb);
