@@ -245,7 +245,7 @@ int launch_attention(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
     }
     if (int rc = launch_after(kern, dim3(blocks), C::THREADS, C::SMEM_BYTES, st, tk, tv, a)) return rc;
     if (!join) return FP4ATTN_OK;
-    return launch_after(paged_join_kernel<OutT, D, HC>, dim3(blocks, a.heads_per_group), 128, 0, st, a);
+    return launch_after(paged_join_kernel<OutT, D, HC>, dim3(blocks, a.heads_per_group), 256, 0, st, a);
 }
 
 template <typename OutT, int D>

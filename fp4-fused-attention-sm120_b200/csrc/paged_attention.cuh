@@ -392,10 +392,6 @@ __global__ void __launch_bounds__(384, 1)
         int g = 0, item = 0;
         bool ok = true;
         for (; ok && t.left > 0; t.next(a), item++, qr.next()) {
-            if (keys_role && lane == 0 && t.tile == 0 && t.hg == 0) {
-                const int len = __ldg(a.seq_lens + t.b);
-                if (len != t.len) record_index_error(kIndexLength, len);
-            }
             const int head = t.hg / a.splits;
             const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift);
             auto page_id = [&](int i) {  // of this lane's page of the part's i-th tile; 0 past its pages
@@ -416,26 +412,36 @@ __global__ void __launch_bounds__(384, 1)
                     ok = false;
                     break;
                 }
+                int pid[8];
+#pragma unroll
+                for (int p = 0; p < 8; p++) pid[p] = __shfl_sync(~0u, id, p);
                 if (keys_role) {
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * C::KROW);
+                    if (ptx::elect_one()) {
+                        ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * C::KROW);
+#pragma unroll
+                        for (int p = 0; p < 8; p++)
+                            if (p < n) ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, pid[p]);
+                    }
                     __syncwarp();
-                    if (lane < n) ptx::tma_load_4d(st + lane * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, id);
                     // Raw scales: 16-byte pieces, page after page.
                     const int piece_shift = shift - 4;  // log2(page / 16): a page has NB << piece_shift pieces
 #pragma unroll
                     for (int c0 = 0; c0 < 8 * C::NB; c0 += 32) {
                         const int c = c0 + lane, p = static_cast<int>(static_cast<unsigned>(c / C::NB) >> piece_shift);
-                        const int pid = __shfl_sync(~0u, id, p & 31);
+                        const int sid = __shfl_sync(~0u, id, p & 31);
                         if (c < 8 * C::NB && p < n)
                             ptx::cp_async16(st + C::K_BYTES + C::V_BYTES + c * 16,
-                                            a.c.k_scales + pid * a.c.k_scales_stride +
+                                            a.c.k_scales + sid * a.c.k_scales_stride +
                                                 static_cast<int64_t>(head) * page * C::NB + (c * 16 - p * page * C::NB));
                     }
                     ptx::cp_async_arrive(&k_full[ring.s]);
                 } else {
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(&v_full[ring.s], n * page * D * 2);
-                    __syncwarp();
-                    if (lane < n) ptx::tma_load_5d(st + C::K_BYTES + lane * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, id);
+                    if (ptx::elect_one()) {
+                        ptx::mbar_arrive_expect_tx(&v_full[ring.s], n * page * D * 2);
+#pragma unroll
+                        for (int p = 0; p < 8; p++)
+                            if (p < n) ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, pid[p]);
+                    }
                 }
                 __syncwarp();
                 id = next_id;
@@ -459,6 +465,10 @@ __global__ void __launch_bounds__(384, 1)
                 }
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(&q_full[qr.s]);
+                if (lane == 0 && t.tile == 0 && t.hg == 0) {
+                    const int len = __ldg(a.seq_lens + t.b);
+                    if (len != t.len) record_index_error(kIndexLength, len);
+                }
             }
         }
         // Every copy issued lands before the block exits.
@@ -521,7 +531,7 @@ __global__ void __launch_bounds__(384, 1)
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) {
+                    if (ptx::elect_one()) {
                         ptx::tc_fence_after();
                         if (i == 0 && u == 0)
 #pragma unroll
@@ -543,28 +553,25 @@ __global__ void __launch_bounds__(384, 1)
                     ring.next();
                 }
                 if (!ok) break;
-                if (lane == 0) {
+                if (ptx::elect_one()) {
                     ptx::tc_commit(&s_full[2 * wg + (j & 1)]);
                     if (i + 1 == n_steps) ptx::tc_commit(&q_empty[qb]);
                 }
             }
         }
-        if (lane == 0) {  // everything issued completes before Tensor Memory is freed
+        if (ptx::elect_one()) {  // everything issued completes before Tensor Memory is freed
             ptx::tc_commit(&drain[0]);
             bounded_drain(&drain[0], 0, 2 * a.timeout_ns);
         }
         __syncwarp();
     } else if (warp == 3) {
         // ------------------------------------------------------------ O^T issuer
-        if (lane == 0) {
+        // (elect.sync, not a lane number: the compiler then knows that one
+        // thread runs this, and an MMA takes 47 cycles to issue instead of 105)
+        if (ptx::elect_one()) {
             constexpr uint32_t idesc_o = ptx::idesc_f16x(128, C::NP, 0, true, true);
-            // V's 16-key steps within a stage, in 16-byte units: page by page, rows within a page.
-            auto v_at = [&](int kk) {
-                return static_cast<uint32_t>((((kk * 16) >> shift) * page * D * 2 + ((kk * 16) & (page - 1)) * C::CB) >> 4);
-            };
-            uint32_t vo[8];
-#pragma unroll
-            for (int kk = 0; kk < 8; kk++) vo[kk] = v_at(kk);
+            // V's 16-key steps within a stage, in 16-byte units: rows within a page, page by page.
+            const int page_shift = shift - 4, page_mask = (1 << page_shift) - 1, page_step = page * D * 2 / 16;
             const uint64_t vd0 = ptx::make_sdesc(ptx::smem_u32(stages + C::K_BYTES), page * C::CB, 8 * C::CB, C::VSW);
             const uint64_t pd0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_P), C::P_BYTES, 8 * C::PROW, C::PSW);
             const uint32_t m_step = static_cast<uint32_t>((128 / C::CHE) * page * C::CB / 16);
@@ -588,20 +595,15 @@ __global__ void __launch_bounds__(384, 1)
                         const uint64_t pd = pd0 + static_cast<uint64_t>((buf * C::U + u) * C::P_BYTES / 16);
                         const uint32_t od = tmem + C::O_COL + buf * C::MT * C::NP;
                         const int keys = t.keys(ti);
-                        if (keys > kPagedTile - 16) {
-#pragma unroll
-                            for (int kk = 0; kk < 8; kk++)
-#pragma unroll
-                                for (int m = 0; m < C::MT; m++)
-                                    ptx::mma_f16_ss(od + m * C::NP, vd + (vo[kk] + m * m_step), pd + kk * C::PROW, idesc_o,
-                                                    (kk > 0 || u > 0) ? 1u : 0u);
-                        } else {
+                        const int steps = max(1, (keys + 15) / 16);
 #pragma unroll 1
-                            for (int kk = 0; kk < max(1, (keys + 15) / 16); kk++)
+                        for (int kk = 0; kk < steps; kk++) {
+                            // 16 keys further within a page, or to the next page.
+                            const uint32_t v = (kk & page_mask) * (16 * C::CB / 16) + (kk >> page_shift) * page_step;
 #pragma unroll
-                                for (int m = 0; m < C::MT; m++)
-                                    ptx::mma_f16_ss(od + m * C::NP, vd + (v_at(kk) + m * m_step), pd + kk * C::PROW, idesc_o,
-                                                    (kk > 0 || u > 0) ? 1u : 0u);
+                            for (int m = 0; m < C::MT; m++)
+                                ptx::mma_f16_ss(od + m * C::NP, vd + (v + m * m_step), pd + kk * C::PROW, idesc_o,
+                                                (kk > 0 || u > 0) ? 1u : 0u);
                         }
                         ptx::tc_commit(&empty[ring.s]);
                         ring.next();
@@ -837,45 +839,70 @@ __global__ void __launch_bounds__(384, 1)
 }
 
 // Block (j, h): head h of the item that attention block j began and others
-// continued: their partial results, in the blocks' order.
+// continued: their partial results, in the blocks' order.  A chain of three
+// loads from memory (what to join, the weights, the parts), so the parts are
+// read by as many threads as there are: kRows of them at once, 16 bytes a
+// thread, and added in shared memory.
 template <typename OutT, int D, int HC>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a)
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedArgs a)
 {
+    constexpr int kRows = 256 / (D / 4) < 8 ? 256 / (D / 4) : 8;
+    __shared__ float weight[kPagedBlocks];
+    __shared__ float red[16];
+    __shared__ float4 sums[kRows][D / 4];
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, h = blockIdx.y;
     ptx::grid_dependency_wait();
     const int4 it = a.p.items[blockIdx.x];
     if (it.x < 0) return;
-    const int h = blockIdx.y, tid = threadIdx.x;
     const int h0 = (it.y % a.splits) * a.heads_per_group;
     if (h >= min(a.heads_per_group, a.group - h0)) return;
-    __shared__ float weight[kPagedBlocks];
-    __shared__ float red[8];
     const int parts = it.z - blockIdx.x + 1;
     auto slot = [&](int p) { return p == 0 ? it.w : 2 * (static_cast<int>(blockIdx.x) + p); };
-    float top = -INFINITY;
-    for (int p = tid; p < parts; p += 128) top = fmaxf(top, a.p.ml[slot(p) * HC + h].x);
-    top = ptx::warp_max(top);
-    if (tid % 32 == 0) red[tid / 32] = top;
+    // The first rows of parts are on their way while the weights are formed.
+    const int r = tid / (D / 4), c = tid % (D / 4);
+    auto part = [&](int p) {
+        return __ldg(reinterpret_cast<const float4*>(a.p.o + (static_cast<int64_t>(slot(p)) * HC + h) * D) + c);
+    };
+    float4 first = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < kRows && r < parts) first = part(r);
+    const float2 ml = tid < parts ? a.p.ml[slot(tid) * HC + h] : make_float2(-INFINITY, 0.f);  // parts <= 148
+    const float wtop = ptx::warp_max(ml.x);
+    if (lane == 0) red[warp] = wtop;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float sum = 0.f;
-    for (int p = tid; p < parts; p += 128) {
-        const float2 ml = a.p.ml[slot(p) * HC + h];
-        const float wgt = ptx::ex2_approx(ml.x - top);
-        weight[p] = wgt;
-        sum += wgt * ml.y;
-    }
+    float top = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) top = fmaxf(top, red[i]);
+    const float wgt = ptx::ex2_approx(ml.x - top);  // 0 for no part
+    if (tid < parts) weight[tid] = wgt;
+    float sum = wgt * ml.y;
+#pragma unroll
     for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(~0u, sum, i);
-    if (tid % 32 == 0) red[4 + tid / 32] = sum;
+    if (lane == 0) red[8 + warp] = sum;
     __syncthreads();
-    sum = (red[4] + red[5]) + (red[6] + red[7]);
-    const int64_t at = static_cast<int64_t>(it.x) * a.q_heads + (it.y / a.splits) * a.group + h0 + h;
-    for (int d = tid; d < D; d += 128) {
-        float o = 0.f;
-#pragma unroll 4
-        for (int p = 0; p < parts; p++) o = fmaf(weight[p], a.p.o[(static_cast<int64_t>(slot(p)) * HC + h) * D + d], o);
-        static_cast<OutT*>(a.out)[at * D + d] = from_float<OutT>(o / sum);
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += red[8 + i];
+    if (r < kRows) {
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = r; p < parts; p += kRows) {
+            const float4 v = p == r ? first : part(p);
+            const float k = weight[p];
+            o.x = fmaf(k, v.x, o.x);
+            o.y = fmaf(k, v.y, o.y);
+            o.z = fmaf(k, v.z, o.z);
+            o.w = fmaf(k, v.w, o.w);
+        }
+        sums[r][c] = o;
     }
-    if (a.lse && tid == 0) a.lse[at] = (top + log2f(sum)) * 0.6931471805599453f;
+    __syncthreads();
+    const int64_t at = static_cast<int64_t>(it.x) * a.q_heads + (it.y / a.splits) * a.group + h0 + h;
+    if (tid < D) {
+        float o = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRows; i++) o += reinterpret_cast<const float*>(sums[i])[tid];
+        static_cast<OutT*>(a.out)[at * D + tid] = from_float<OutT>(__fdividef(o, sum));
+    }
+    if (a.lse && tid == 0) a.lse[at] = (top + __log2f(sum)) * 0.6931471805599453f;
 }
 
 }  // namespace fp4attn
