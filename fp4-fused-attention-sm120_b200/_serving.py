@@ -36,24 +36,44 @@ def declare(L) -> None:
     L.fp4attn_paged_attention_workspace_size.restype = sz
 
 
-lib, check, torch, scale_mode = _fa.lib, _fa._check, _fa._torch, _fa._scale_mode
+lib, check, scale_mode = _fa.lib, _fa._check, _fa._scale_mode
+I2, I3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+_T = None
+_CODES = {}
 
 
-def dtype_code(t) -> int:
-    return _fa._dtype_code(t)
+def torch():
+    """torch, imported on the first call (these functions run once a layer and
+    token, so what they look up is kept)."""
+    global _T
+    if _T is None:
+        _T = _fa._torch()
+        _CODES.update({_T.float16: F16, _T.float32: F32})
+    return _T
+
+
+def dtype_code(dtype) -> int:
+    torch()
+    code = _CODES.get(dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}; use float16 or float32")
+    return code
 
 
 def check_index(t, name, device):
-    if t.dtype != torch().int32 or t.device != device:
+    if t.dtype is not torch().int32 or t.device != device:
         raise ValueError(f"{name} must be an int32 tensor on {device}")
 
 
 def check_table(table, device, head_dim):
-    if (table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch().float32 or table.device != device or
+    """(pointer, rotary_dim, positions) of a rotary table."""
+    shape = table.shape
+    if (len(shape) != 3 or shape[2] != 2 or table.dtype is not torch().float32 or table.device != device or
             not table.is_contiguous()):
         raise ValueError(f"table must be a contiguous float32 [positions, rotary_dim / 2, 2] tensor on {device}")
-    if 2 * table.shape[1] > head_dim:
-        raise ValueError(f"the table's rotary_dim {2 * table.shape[1]} exceeds head_dim {head_dim}")
+    if 2 * shape[1] > head_dim:
+        raise ValueError(f"the table's rotary_dim {2 * shape[1]} exceeds head_dim {head_dim}")
+    return table.data_ptr(), 2 * shape[1], shape[0]
 
 
 _HERE = contextlib.nullcontext()
@@ -71,5 +91,6 @@ def on(device, stream):
     return _HERE if device.index == T.cuda.current_device() else T.cuda.device(device)
 
 
-def stream_ptr() -> int:
-    return torch().cuda.current_stream().cuda_stream
+def stream_ptr(device) -> int:
+    """The current stream of a device, as the library takes it."""
+    return _T._C._cuda_getCurrentRawStream(device.index)

@@ -67,27 +67,31 @@ class PagedCache:
                    torch.empty(shape + (head_dim,), dtype=torch.float16, device=device))
 
 
-def _check_block_table(block_table, cache):
-    sv.check_index(block_table, "block_table", cache.device)
-    if block_table.dim() != 2 or block_table.shape[1] < 1 or block_table.stride(1) != 1:
+def _check_block_table(block_table, device):
+    """(pointer, row stride, sequences, pages) of a block table."""
+    sv.check_index(block_table, "block_table", device)
+    shape, strides = block_table.shape, block_table.stride()
+    if len(shape) != 2 or shape[1] < 1 or strides[1] != 1:
         raise ValueError("block_table must be [sequences, pages] with contiguous rows")
-    n, pages = block_table.shape
-    return block_table.data_ptr(), max(block_table.stride(0), pages) if n < 2 else block_table.stride(0), n, pages
+    n, pages = shape
+    return block_table.data_ptr(), strides[0] if n > 1 else pages, n, pages
 
 
-def _check_vector(t, name, n, cache):
-    sv.check_index(t, name, cache.device)
-    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+def _check_vector(t, name, n, device):
+    sv.check_index(t, name, device)
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a contiguous int32 [{n}] tensor")
     return t.data_ptr()
 
 
 def _check_rows(t, name, tokens, heads, cache, dtype):
-    if (t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != cache.head_dim or (heads and t.shape[1] != heads) or
-            t.device != cache.device or t.dtype != dtype or t.stride(2) != 1):
+    """(token, head) strides of a [tokens, heads, head_dim] tensor; heads=None: any number."""
+    shape, strides = t.shape, t.stride()
+    if (len(shape) != 3 or shape[0] != tokens or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads) or
+            t.device != cache.device or t.dtype is not dtype or strides[2] != 1):
         raise ValueError(f"{name} must be a [{tokens}, {heads or 'heads'}, {cache.head_dim}] {dtype} tensor on "
                          f"{cache.device} with a contiguous last dimension")
-    return (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+    return sv.I2(strides[0], strides[1])
 
 
 def cache_append(cache, K, V, block_table, positions, seq_ids=None, Q=None, table=None, interleaved=False,
@@ -100,24 +104,23 @@ def cache_append(cache, K, V, block_table, positions, seq_ids=None, Q=None, tabl
     the queries rotated the same way, contiguous.  No two tokens of a call may
     have the same place in the cache."""
     torch = sv.torch()
-    tokens = K.shape[0]
-    ks = _check_rows(K, "K", tokens, cache.kv_heads, cache, K.dtype)
-    vs = _check_rows(V, "V", tokens, cache.kv_heads, cache, K.dtype)
-    qs = None if Q is None else _check_rows(Q, "Q", tokens, 0, cache, K.dtype)
-    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, cache)
-    pos = _check_vector(positions, "positions", tokens, cache)
-    ids = None if seq_ids is None else _check_vector(seq_ids, "seq_ids", tokens, cache)
-    if table is not None:
-        sv.check_table(table, cache.device, cache.head_dim)
-    code, rule = sv.dtype_code(K), sv.scale_mode(scale_mode)
-    with sv.on(cache.device, stream):
-        out = None if Q is None else torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
+    tokens, dtype, device = K.shape[0], K.dtype, cache.device
+    code, rule = sv.dtype_code(dtype), sv.scale_mode(scale_mode)
+    ks = _check_rows(K, "K", tokens, cache.kv_heads, cache, dtype)
+    vs = _check_rows(V, "V", tokens, cache.kv_heads, cache, dtype)
+    qs = None if Q is None else _check_rows(Q, "Q", tokens, None, cache, dtype)
+    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, device)
+    pos = _check_vector(positions, "positions", tokens, device)
+    ids = None if seq_ids is None else _check_vector(seq_ids, "seq_ids", tokens, device)
+    tab = (None, 0, 0) if table is None else sv.check_table(table, device, cache.head_dim)
+    with sv.on(device, stream):
+        out, q_ptr, out_ptr, q_heads = None, None, None, 0
+        if Q is not None:
+            out, q_ptr, q_heads = torch.empty(Q.shape, dtype=dtype, device=device), Q.data_ptr(), Q.shape[1]
+            out_ptr = out.data_ptr()
         sv.check(sv.lib().fp4attn_cache_append(
-            cache.struct, K.data_ptr(), V.data_ptr(), None if Q is None else Q.data_ptr(),
-            None if Q is None else out.data_ptr(), code, tokens, 0 if Q is None else Q.shape[1], ks, vs, qs,
-            bt, bt_stride, seqs, max_pages, ids, pos, None if table is None else table.data_ptr(),
-            0 if table is None else 2 * table.shape[1], 0 if table is None else table.shape[0], int(interleaved), rule,
-            sv.stream_ptr()), "fp4attn_cache_append")
+            cache.struct, K.data_ptr(), V.data_ptr(), q_ptr, out_ptr, code, tokens, q_heads, ks, vs, qs, bt, bt_stride,
+            seqs, max_pages, ids, pos, *tab, interleaved, rule, sv.stream_ptr(device)), "fp4attn_cache_append")
     return out
 
 
@@ -128,16 +131,18 @@ def cache_gather(cache, block_table, starts, lengths, max_length, heads=None, dt
     (default: the cache's) repeats each key/value head for its query heads, as
     fused_fp4_attention wants them."""
     torch = sv.torch()
-    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, cache)
-    st = None if starts is None else _check_vector(starts, "starts", seqs, cache)
-    ln = _check_vector(lengths, "lengths", seqs, cache)
+    device = cache.device
+    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, device)
+    st = None if starts is None else _check_vector(starts, "starts", seqs, device)
+    ln = _check_vector(lengths, "lengths", seqs, device)
     heads = cache.kv_heads if heads is None else heads
     dtype = dtype or torch.float16
-    with sv.on(cache.device, stream):
-        K, V = (torch.empty((seqs, heads, max_length, cache.head_dim), dtype=dtype, device=cache.device)
-                for _ in range(2))
+    code = sv.dtype_code(dtype)
+    with sv.on(device, stream):
+        K = torch.empty((seqs, heads, max_length, cache.head_dim), dtype=dtype, device=device)
+        V = torch.empty_like(K)
         sv.check(sv.lib().fp4attn_cache_gather(cache.struct, bt, bt_stride, seqs, max_pages, st, ln, max_length, heads,
-                                               K.data_ptr(), V.data_ptr(), sv.dtype_code(K), sv.stream_ptr()),
+                                               K.data_ptr(), V.data_ptr(), code, sv.stream_ptr(device)),
                  "fp4attn_cache_gather")
     return K, V
 
@@ -150,30 +155,35 @@ def paged_attention_workspace_size(cache, batch, heads):
 
 def _attend(Q, cache, block_table, seq_lens, softmax_scale, scale_mode, out_dtype, out, with_lse, workspace, stream):
     torch = sv.torch()
-    qs = _check_rows(Q, "Q", Q.shape[0], 0, cache, Q.dtype)
+    dtype, device = Q.dtype, cache.device
+    code, rule = sv.dtype_code(dtype), sv.scale_mode(scale_mode)
+    qs = _check_rows(Q, "Q", Q.shape[0], None, cache, dtype)
     B, H, D = Q.shape
-    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, cache)
+    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, device)
     if seqs != B:
         raise ValueError(f"block_table has {seqs} rows for {B} queries")
-    ln = _check_vector(seq_lens, "seq_lens", B, cache)
-    if out is not None and (out.shape != Q.shape or not out.is_contiguous() or out.device != Q.device or
-                            (out_dtype is not None and out.dtype != out_dtype)):
-        raise ValueError("out must be contiguous with Q's shape, on its device")
-    if workspace is not None and (workspace.device != Q.device or workspace.dtype != torch.uint8 or
+    ln = _check_vector(seq_lens, "seq_lens", B, device)
+    if out is None:
+        out_code = code if out_dtype is None else sv.dtype_code(out_dtype)
+    else:
+        out_code = sv.dtype_code(out.dtype)
+        if (out.shape != Q.shape or not out.is_contiguous() or out.device != device or
+                (out_dtype is not None and out.dtype != out_dtype)):
+            raise ValueError("out must be contiguous with Q's shape, on its device")
+    if workspace is not None and (workspace.device != device or workspace.dtype is not torch.uint8 or
                                   not workspace.is_contiguous()):
         raise ValueError("workspace must be a contiguous uint8 tensor on Q's device")
-    code, rule = sv.dtype_code(Q), sv.scale_mode(scale_mode)
-    with sv.on(cache.device, stream):
+    with sv.on(device, stream):
         if out is None:
-            out = torch.empty((B, H, D), dtype=out_dtype or Q.dtype, device=Q.device)
-        lse = torch.empty((B, H), dtype=torch.float32, device=Q.device) if with_lse else None
+            out = torch.empty((B, H, D), dtype=out_dtype or dtype, device=device)
+        lse = torch.empty((B, H), dtype=torch.float32, device=device) if with_lse else None
         if workspace is None:
-            size = max(1, paged_attention_workspace_size(cache, B, H))
-            workspace = torch.empty(size, dtype=torch.uint8, device=Q.device)
+            workspace = torch.empty(max(1, paged_attention_workspace_size(cache, B, H)), dtype=torch.uint8,
+                                    device=device)
         sv.check(sv.lib().fp4attn_paged_attention(
-            cache.struct, Q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), code,
-            sv.dtype_code(out), B, H, qs, bt, bt_stride, max_pages, ln, float(softmax_scale or 0.0), rule,
-            workspace.data_ptr(), workspace.numel(), sv.stream_ptr()), "fp4attn_paged_attention")
+            cache.struct, Q.data_ptr(), out.data_ptr(), lse.data_ptr() if with_lse else None, code, out_code, B, H, qs,
+            bt, bt_stride, max_pages, ln, softmax_scale or 0.0, rule, workspace.data_ptr(), workspace.numel(),
+            sv.stream_ptr(device)), "fp4attn_paged_attention")
     return out, lse
 
 
@@ -205,28 +215,38 @@ def copy_pages(caches, src, dst, stream=None):
     layers and 64 pages (fp4attn_copy_pages).  src and dst: sequences of ints or
     CPU integer tensors.  No page may be written twice, or both read and
     written."""
-    torch = sv.torch()
     caches = list(caches)
     if not caches:
         return
-    if any(c.device != caches[0].device for c in caches):
-        raise ValueError("the caches must be on one device")
-    src, dst = (torch.as_tensor(t) for t in (src, dst))
-    for name, t in (("src", src), ("dst", dst)):
-        if t.numel() and (t.is_cuda or t.dim() != 1 or t.is_floating_point() or t.dtype == torch.bool):
-            raise ValueError(f"{name} must be page numbers in host memory")
-    if src.numel() != dst.numel():
+    device = caches[0].device
+    src, dst = _page_numbers(src, "src"), _page_numbers(dst, "dst")
+    n = src.shape[0]
+    if n != dst.shape[0]:
         raise ValueError("src and dst differ in length")
-    if src.numel() == 0:
-        return
-    # (numbers that int32 would cut are refused here; the library checks the rest)
-    if max(int(src.max()), int(dst.max())) > 0x7FFFFFFF or min(int(src.min()), int(dst.min())) < 0:
-        raise ValueError("page number out of range")
-    src, dst = src.to(torch.int32).contiguous(), dst.to(torch.int32).contiguous()
-    structs = (sv.CacheStruct * len(caches))(*(c.struct for c in caches))
-    with sv.on(caches[0].device, stream):
-        sv.check(sv.lib().fp4attn_copy_pages(structs, len(caches), src.data_ptr(), dst.data_ptr(), src.numel(),
-                                             sv.stream_ptr()), "fp4attn_copy_pages")
+    structs = (sv.CacheStruct * len(caches))(*[c.struct for c in caches])
+    for c in caches:
+        if c.device != device:
+            raise ValueError("the caches must be on one device")
+    with sv.on(device, stream):
+        sv.check(sv.lib().fp4attn_copy_pages(structs, len(caches), src.data_ptr(), dst.data_ptr(), n,
+                                             sv.stream_ptr(device)), "fp4attn_copy_pages")
+
+
+def _page_numbers(pages, name):
+    """A contiguous int32 CPU tensor of page numbers (their range is checked by the library)."""
+    torch = sv.torch()
+    if not isinstance(pages, torch.Tensor):
+        pages = torch.tensor(pages, dtype=torch.int64)
+    if pages.dtype is not torch.int32:
+        if pages.dtype is not torch.int64:
+            raise ValueError(f"{name} must be int32 or int64")
+        narrow = pages.to(torch.int32)
+        if not torch.equal(narrow.to(torch.int64), pages):
+            raise ValueError(f"{name}: page number out of range")
+        pages = narrow
+    if pages.dim() != 1 or pages.is_cuda:
+        raise ValueError(f"{name} must be page numbers in host memory")
+    return pages.contiguous()
 
 
 class PagePool:

@@ -79,7 +79,7 @@ def rotary_table(max_positions, rotary_dim, base=10000.0, scaling=None, factor=1
     with sv.on(device, stream):
         table = torch.empty((max_positions, rotary_dim // 2, 2), dtype=torch.float32, device=device)
         sv.check(sv.lib().fp4attn_rotary_table(arr, len(freqs), max_positions, table_factor, table.data_ptr(),
-                                               sv.stream_ptr()), "fp4attn_rotary_table")
+                                               sv.stream_ptr(device)), "fp4attn_rotary_table")
     return table
 
 
@@ -92,13 +92,15 @@ def rotary(x, table, positions=None, interleaved=False, inverse=False, out=None,
     interleaved: pairs (2j, 2j + 1) instead of (j, j + rotary_dim / 2).
     inverse: turn back, which is the gradient's rotation."""
     torch = sv.torch()
-    if x.dim() != 4 or not x.is_cuda or x.stride(3) != 1:
+    device, dtype, strides = x.device, x.dtype, x.stride()
+    if len(strides) != 4 or not x.is_cuda or strides[3] != 1:
         raise ValueError("x must be a [batch, heads, seq, head_dim] CUDA tensor with a contiguous last dimension")
     B, H, S, D = x.shape
-    sv.check_table(table, x.device, D)
+    code = sv.dtype_code(dtype)
+    table_ptr, rotary_dim, max_positions = sv.check_table(table, device, D)
     pos_ptr, pos_stride = None, 0
     if positions is not None:
-        sv.check_index(positions, "positions", x.device)
+        sv.check_index(positions, "positions", device)
         if positions.dim() == 2 and positions.shape == (B, S):
             pos_stride = positions.stride(0)
         elif positions.shape != (S,):
@@ -106,17 +108,15 @@ def rotary(x, table, positions=None, interleaved=False, inverse=False, out=None,
         if S > 1 and positions.stride(-1) != 1:
             raise ValueError("positions must be contiguous along seq")
         pos_ptr = positions.data_ptr()
-    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or
-                            out.stride(3) != 1):
+    if out is not None and (out.shape != x.shape or out.dtype != dtype or out.device != device or out.stride(3) != 1):
         raise ValueError("out must have x's shape, dtype and device, and a contiguous last dimension")
-    i64 = ctypes.c_int64 * 3
-    with sv.on(x.device, stream):
+    with sv.on(device, stream):
         if out is None:
-            out = torch.empty((B, H, S, D), dtype=x.dtype, device=x.device)
+            out = torch.empty((B, H, S, D), dtype=dtype, device=device)
         sv.check(sv.lib().fp4attn_rotary(
-            x.data_ptr(), out.data_ptr(), sv.dtype_code(x), B, H, S, D, i64(*x.stride()[:3]), i64(*out.stride()[:3]),
-            table.data_ptr(), 2 * table.shape[1], table.shape[0], pos_ptr, pos_stride, int(interleaved), int(inverse),
-            sv.stream_ptr()), "fp4attn_rotary")
+            x.data_ptr(), out.data_ptr(), code, B, H, S, D, sv.I3(*strides[:3]), sv.I3(*out.stride()[:3]), table_ptr,
+            rotary_dim, max_positions, pos_ptr, pos_stride, interleaved, inverse, sv.stream_ptr(device)),
+            "fp4attn_rotary")
     return out
 
 
