@@ -305,6 +305,30 @@ static __device__ __noinline__ uint32_t quantize_query(const void* q, int64_t at
     return sb == 255u ? 254u : sb;
 }
 
+// copy(p) for pages 0 .. n - 1 of a tile, by one elected thread.  A tile's
+// whole number of pages (1, 2, 4 or 8) goes without a condition on each copy:
+// with one, a copy took 85 cycles to issue instead of 20.
+template <typename F>
+__device__ __forceinline__ void each_page(int n, F copy)
+{
+    if (n == 8) {
+#pragma unroll
+        for (int p = 0; p < 8; p++) copy(p);
+    } else if (n == 4) {
+#pragma unroll
+        for (int p = 0; p < 4; p++) copy(p);
+    } else if (n == 2) {
+        copy(0);
+        copy(1);
+    } else if (n == 1) {
+        copy(0);
+    } else {
+#pragma unroll
+        for (int p = 0; p < 7; p++)
+            if (p < n) copy(p);
+    }
+}
+
 template <typename OutT, int D, int HC>
 __global__ void __launch_bounds__(384, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -418,9 +442,7 @@ __global__ void __launch_bounds__(384, 1)
                 if (keys_role) {
                     if (ptx::elect_one()) {
                         ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * C::KROW);
-#pragma unroll
-                        for (int p = 0; p < 8; p++)
-                            if (p < n) ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, pid[p]);
+                        each_page(n, [&](int p) { ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, pid[p]); });
                     }
                     __syncwarp();
                     // Raw scales: 16-byte pieces, page after page.
@@ -438,9 +460,9 @@ __global__ void __launch_bounds__(384, 1)
                 } else {
                     if (ptx::elect_one()) {
                         ptx::mbar_arrive_expect_tx(&v_full[ring.s], n * page * D * 2);
-#pragma unroll
-                        for (int p = 0; p < 8; p++)
-                            if (p < n) ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, pid[p]);
+                        each_page(n, [&](int p) {
+                            ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, pid[p]);
+                        });
                     }
                 }
                 __syncwarp();
