@@ -37,9 +37,7 @@ enum ServingSite : int {
     kPagedKFull = 1,
     kPagedVFull,
     kPagedEmpty,
-    kPagedScales,
     kPagedQFull,
-    kPagedQEmpty,
     kPagedSFull,
     kPagedSFree,
     kPagedPFull,

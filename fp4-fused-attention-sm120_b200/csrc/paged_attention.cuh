@@ -27,16 +27,16 @@
 // and paged_join_kernel joins them, in order, so results repeat bit for bit.
 //
 // Roles (384 threads):
-//   warp 0      key producer: codes by TMA (a lane per page of the tile), raw
-//               scales by cp.async, into a ring of stages.
-//   warp 1      value producer: V by TMA, a lane per page; and the queries:
-//               quantises each item's query heads, some tiles ahead.
+//   warp 0      key producer (one thread): a page's codes by TMA, its raw
+//               scales by a bulk copy, into a ring of stages.
+//   warp 1      value producer (one thread): a page's V by TMA.
 //   warp 2      S^T issuer: brings the scales into the tensor core's layout,
 //               then one thread issues the MMAs.
 //   warp 3      O^T issuer (one thread).
 //   warps 4-11  two softmax warpgroups, which take the items in turn, so that
 //               one starts an item while the other finishes the one before:
-//               thread = key (row of S^T), then head-dim row of O^T.
+//               thread = key (row of S^T), then head-dim row of O^T.  Each
+//               quantises its own item's queries first.
 // A single thread runs a dependent instruction in about six cycles and passes
 // a ready barrier in about a hundred, and a tile has some 900 (head_dim 64) to
 // 1,800 cycles (128) of the memory's time: one thread that issued both MMAs
@@ -102,11 +102,10 @@ struct PagedCfg {
     static constexpr int STAGE = K_BYTES + V_BYTES + S_BYTES;
     static constexpr int OFF_P = 0;                                  // [2][U][128 keys][PROW]
     static constexpr int P_BYTES = kPagedTile * PROW;
-    static constexpr int QBUFS = 4;                                  // items whose queries may be ready ahead
-    static constexpr int OFF_Q = OFF_P + 2 * U * P_BYTES;            // [QBUFS][NS rows][KROW]
+    static constexpr int OFF_Q = OFF_P + 2 * U * P_BYTES;            // [2 warpgroups][NS rows][KROW]
     static constexpr int Q_BYTES = align1k(NS * KROW);
-    static constexpr int OFF_QSF = OFF_Q + QBUFS * Q_BYTES;          // [QBUFS][ATOMS][512]
-    static constexpr int OFF_KSF = OFF_QSF + QBUFS * ATOMS * 512;    // [2][U][ATOMS][512]
+    static constexpr int OFF_QSF = OFF_Q + 2 * Q_BYTES;              // [2][ATOMS][512]
+    static constexpr int OFF_KSF = OFF_QSF + 2 * ATOMS * 512;        // [2][U][ATOMS][512]
     static constexpr int OFF_STAGE = align1k(OFF_KSF + 2 * U * ATOMS * 512);
     // The O^T MMA reads 128 rows (head-dim columns) of V: past head_dim it
     // reads on into what follows; those rows of O^T are not used.
@@ -339,13 +338,12 @@ __global__ void __launch_bounds__(384, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_MISC);
-    uint64_t* k_full = bars;               // [8] codes (TMA) and scales (cp.async, 32) of a stage landed
+    uint64_t* k_full = bars;               // [8] codes and scales of a stage landed
     uint64_t* v_full = k_full + 8;         // [8] values landed
     uint64_t* empty = v_full + 8;          // [8] the stage's MMAs are done (commit)
-    uint64_t* q_full = empty + 8;          // [4] query codes and scales written (32)
-    uint64_t* q_empty = q_full + 4;        // [4] the item's S^T MMAs are done (commit)
+    uint64_t* q_full = empty + 8;          // [2] an item's query codes and scales written (128), by warpgroup
     // (these by step)
-    uint64_t* s_full = q_empty + 4;        // [2][2] S^T computed (commit); by warpgroup, see below
+    uint64_t* s_full = q_full + 2;        // [2][2] S^T computed (commit); by warpgroup, see below
     uint64_t* s_free = s_full + 4;         // [2] S^T in registers (128)
     uint64_t* p_full = s_free + 2;         // [2] P written (128)
     uint64_t* o_full = p_full + 2;         // [2] O^T computed, P read (commit)
@@ -360,15 +358,12 @@ __global__ void __launch_bounds__(384, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; i++) {
-            ptx::mbar_init(&k_full[i], 1 + 32);
+            ptx::mbar_init(&k_full[i], 1);
             ptx::mbar_init(&v_full[i], 1);
             ptx::mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < C::QBUFS; i++) {
-            ptx::mbar_init(&q_full[i], 32);
-            ptx::mbar_init(&q_empty[i], 1);
-        }
         for (int i = 0; i < 2; i++) {
+            ptx::mbar_init(&q_full[i], 128);
             ptx::mbar_init(&s_full[i], 1);
             ptx::mbar_init(&s_full[2 + i], 1);
             ptx::mbar_init(&s_free[i], 128);
@@ -387,10 +382,10 @@ __global__ void __launch_bounds__(384, 1)
         ptx::tmem_relinquish();
     }
     // Query rows past the group's heads and blocks past head_dim: codes 0,
-    // scale 1, for all buffers.
-    for (int i = threadIdx.x; i < C::QBUFS * C::Q_BYTES / 16; i += C::THREADS)
+    // scale 1, for both buffers.
+    for (int i = threadIdx.x; i < 2 * C::Q_BYTES / 16; i += C::THREADS)
         reinterpret_cast<uint4*>(smem + C::OFF_Q)[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = threadIdx.x; i < C::QBUFS * C::ATOMS * 32; i += C::THREADS)
+    for (int i = threadIdx.x; i < 2 * C::ATOMS * 32; i += C::THREADS)
         reinterpret_cast<uint4*>(smem + C::OFF_QSF)[i] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
     ptx::fence_proxy_async_smem();
     // Everything before this overlaps the grid before this one in the stream.
@@ -411,94 +406,59 @@ __global__ void __launch_bounds__(384, 1)
     if (warp <= 1) {
         // ------------------------------------------------------------ producers
         const bool keys_role = warp == 0;
-        Ring<C::STAGES> ring;
-        Ring<C::QBUFS> qr;
-        int g = 0, item = 0;
-        bool ok = true;
-        for (; ok && t.left > 0; t.next(a), item++, qr.next()) {
-            const int head = t.hg / a.splits;
-            const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift);
-            auto page_id = [&](int i) {  // of this lane's page of the part's i-th tile; 0 past its pages
-                int id = 0;
-                if ((lane << shift) < t.keys(i)) id = __ldg(row + ((i * kPagedTile) >> shift) + lane);
-                return id;
-            };
-            int id = page_id(0);
-            for (int i = 0; i < t.n; i++, g++, ring.next()) {
-                const int next_id = i + 1 < t.n ? page_id(i + 1) : 0;
-                const int n = (t.keys(i) + page - 1) >> shift;  // pages of this tile
-                if (id < 0 || id >= a.c.pages) {
-                    if (keys_role) record_index_error(kIndexPage, id);
-                    id = 0;
-                }
-                uint8_t* st = stages + ring.s * C::STAGE;
-                if (g >= C::STAGES && !__all_sync(~0u, bounded_wait(&empty[ring.s], ring.parity ^ 1u, w, kPagedEmpty))) {
-                    ok = false;
-                    break;
-                }
-                int pid[8];
+        if (ptx::elect_one()) {
+            Ring<C::STAGES> ring;
+            int g = 0;
+            bool ok = true;
+            for (; ok && t.left > 0; t.next(a)) {
+                const int head = t.hg / a.splits;
+                const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift);
+                int id[8];  // the tile's pages (those of the next are loaded a tile ahead)
+                auto load_ids = [&](int i, int (&to)[8]) {
+                    const int keys = i < t.n ? t.keys(i) : 0;
+                    const int32_t* from = row + ((i * kPagedTile) >> shift);
 #pragma unroll
-                for (int p = 0; p < 8; p++) pid[p] = __shfl_sync(~0u, id, p);
-                if (keys_role) {
-                    if (ptx::elect_one()) {
-                        ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * C::KROW);
-                        each_page(n, [&](int p) { ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, pid[p]); });
-                    }
-                    __syncwarp();
-                    // Raw scales: 16-byte pieces, page after page.
-                    const int piece_shift = shift - 4;  // log2(page / 16): a page has NB << piece_shift pieces
+                    for (int p = 0; p < 8; p++) to[p] = (p << shift) < keys ? __ldg(from + p) : 0;
+                };
+                load_ids(0, id);
+                for (int i = 0; i < t.n; i++, g++, ring.next()) {
+                    int next[8];
+                    load_ids(i + 1, next);
+                    const int n = (t.keys(i) + page - 1) >> shift;
 #pragma unroll
-                    for (int c0 = 0; c0 < 8 * C::NB; c0 += 32) {
-                        const int c = c0 + lane, p = static_cast<int>(static_cast<unsigned>(c / C::NB) >> piece_shift);
-                        const int sid = __shfl_sync(~0u, id, p & 31);
-                        if (c < 8 * C::NB && p < n)
-                            ptx::cp_async16(st + C::K_BYTES + C::V_BYTES + c * 16,
-                                            a.c.k_scales + sid * a.c.k_scales_stride +
-                                                static_cast<int64_t>(head) * page * C::NB + (c * 16 - p * page * C::NB));
+                    for (int p = 0; p < 8; p++)
+                        if (static_cast<unsigned>(id[p]) >= static_cast<unsigned>(a.c.pages)) {
+                            record_index_error(kIndexPage, id[p]);
+                            id[p] = 0;
+                        }
+                    uint8_t* st = stages + ring.s * C::STAGE;
+                    if (g >= C::STAGES && !bounded_wait(&empty[ring.s], ring.parity ^ 1u, w, kPagedEmpty)) {
+                        ok = false;
+                        break;
                     }
-                    ptx::cp_async_arrive(&k_full[ring.s]);
-                } else {
-                    if (ptx::elect_one()) {
+                    if (keys_role) {
+                        ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * (C::KROW + C::NB));
+                        const uint8_t* scales = a.c.k_scales + static_cast<int64_t>(head) * page * C::NB;
+                        each_page(n, [&](int p) {
+                            ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, id[p]);
+                            ptx::bulk_load(st + C::K_BYTES + C::V_BYTES + p * page * C::NB, scales + id[p] * a.c.k_scales_stride,
+                                           page * C::NB, &k_full[ring.s]);
+                        });
+                    } else {
                         ptx::mbar_arrive_expect_tx(&v_full[ring.s], n * page * D * 2);
                         each_page(n, [&](int p) {
-                            ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, pid[p]);
+                            ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, id[p]);
                         });
                     }
-                }
-                __syncwarp();
-                id = next_id;
-                if (keys_role || i > 0) continue;
-                // This item's queries.
-                if (item >= C::QBUFS && !__all_sync(~0u, bounded_wait(&q_empty[qr.s], qr.parity ^ 1u, w, kPagedQEmpty))) {
-                    ok = false;
-                    g++;  // (the tile just issued is in flight)
-                    break;
-                }
-                const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
-                const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(head) * a.group + h0) * a.qh;
-                for (int k = lane; k < nh * C::NB; k += 32) {
-                    const int r = k / C::NB, blk = k % C::NB;
-                    const int64_t at = q0 + r * a.qh + blk * 32;
-                    uint4 packed;
-                    const uint32_t sb = quantize_query(a.q, at, a.q_half, a.ocp, &packed);
-                    const int sw = C::KROW == 32 ? (r >> 2) & 1 : C::KROW == 64 ? (r >> 1) & 3 : r & 7;
-                    *reinterpret_cast<uint4*>(smem + C::OFF_Q + qr.s * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16)) = packed;
-                    smem[C::OFF_QSF + (qr.s * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb);
-                }
-                ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive(&q_full[qr.s]);
-                if (lane == 0 && t.tile == 0 && t.hg == 0) {
-                    const int len = __ldg(a.seq_lens + t.b);
-                    if (len != t.len) record_index_error(kIndexLength, len);
+#pragma unroll
+                    for (int p = 0; p < 8; p++) id[p] = next[p];
                 }
             }
-        }
-        // Every copy issued lands before the block exits.
-        ptx::cp_async_wait_all();
-        if (lane == 0)
+            // Every copy issued lands before the block exits.
             for (int i = max(0, g - C::STAGES); i < g; i++)
                 bounded_drain(keys_role ? &k_full[i % C::STAGES] : &v_full[i % C::STAGES],
                               static_cast<uint32_t>(i / C::STAGES) & 1u, 2 * a.timeout_ns);
+        }
         __syncwarp();
     } else if (warp == 2) {
         // ------------------------------------------------------------ S^T issuer
@@ -508,14 +468,13 @@ __global__ void __launch_bounds__(384, 1)
         const uint64_t sfa0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_KSF), 0, 128, ptx::kSwizzleNone);
         const uint64_t sfb0 = ptx::make_sdesc(ptx::smem_u32(smem + C::OFF_QSF), 0, 128, ptx::kSwizzleNone);
         Ring<C::STAGES> ring;
-        Ring<C::QBUFS> qr;
         // A warpgroup waits for its own tiles only, and a barrier's parity tells
         // a phase from the one before it alone: so each has its own barriers,
         // used in the order of its tiles.
         int g = 0, own[2] = {0, 0};
         bool ok = true;
-        for (int wg = 0; ok && t.left > 0; t.next(a), qr.next(), wg ^= 1) {
-            const int qb = qr.s;
+        for (int item = 0; ok && t.left > 0; t.next(a), item++) {
+            const int wg = item & 1;
             int j = own[wg];
             const int n_steps = (t.n + C::U - 1) / C::U;
             own[wg] += n_steps;
@@ -523,7 +482,7 @@ __global__ void __launch_bounds__(384, 1)
                 const int buf = g & 1;
                 // S^T and the scale atoms of step g - 2 have been read.
                 bool go = g < 2 || bounded_wait(&s_free[buf], static_cast<uint32_t>((g - 2) / 2) & 1u, w, kPagedSFree);
-                if (i == 0) go = bounded_wait(&q_full[qb], qr.parity, w, kPagedQFull) && go;
+                if (i == 0) go = bounded_wait(&q_full[wg], static_cast<uint32_t>(item / 2) & 1u, w, kPagedQFull) && go;
 #pragma unroll
                 for (int u = 0; u < C::U; u++) {
                     if (u > 0 && i * C::U + u >= t.n) break;
@@ -558,11 +517,11 @@ __global__ void __launch_bounds__(384, 1)
                         if (i == 0 && u == 0)
 #pragma unroll
                             for (int k = 0; k < C::ATOMS; k++)
-                                ptx::tc_cp_32x128b_warpx4(tmem + C::SFB_COL + 4 * k, sfb0 + (qb * C::ATOMS + k) * (512 / 16));
+                                ptx::tc_cp_32x128b_warpx4(tmem + C::SFB_COL + 4 * k, sfb0 + (wg * C::ATOMS + k) * (512 / 16));
 #pragma unroll
                         for (int k = 0; k < C::ATOMS; k++)
                             ptx::tc_cp_32x128b_warpx4(tmem + C::SFA_COL + 4 * k, sfa0 + ((buf * C::U + u) * C::ATOMS + k) * (512 / 16));
-                        const uint64_t kd = kd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16)), qd = qd0 + qb * (C::Q_BYTES / 16);
+                        const uint64_t kd = kd0 + static_cast<uint64_t>(ring.s * (C::STAGE / 16)), qd = qd0 + wg * (C::Q_BYTES / 16);
 #pragma unroll
                         for (int kk = 0; kk < C::KSTEPS; kk++) {
                             const uint32_t id = 2u * (kk & 1);
@@ -575,10 +534,7 @@ __global__ void __launch_bounds__(384, 1)
                     ring.next();
                 }
                 if (!ok) break;
-                if (ptx::elect_one()) {
-                    ptx::tc_commit(&s_full[2 * wg + (j & 1)]);
-                    if (i + 1 == n_steps) ptx::tc_commit(&q_empty[qb]);
-                }
+                if (ptx::elect_one()) ptx::tc_commit(&s_full[2 * wg + (j & 1)]);
             }
         }
         if (ptx::elect_one()) {  // everything issued completes before Tensor Memory is freed
@@ -663,6 +619,26 @@ __global__ void __launch_bounds__(384, 1)
                 for (int i = t.n % C::STAGES; i > 0; i--) ring.next();
                 ring.parity ^= static_cast<uint32_t>(t.n / C::STAGES) & 1u;
                 continue;
+            }
+            const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
+            // This item's queries, while the other warpgroup has the item before.
+            // (S^T of this warpgroup's last item, the buffer's last use, is computed.)
+            {
+                const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(t.hg / a.splits) * a.group + h0) * a.qh;
+                for (int k = row; k < nh * C::NB; k += 128) {
+                    const int r = k / C::NB, blk = k % C::NB;
+                    uint4 packed;
+                    const uint32_t sb = quantize_query(a.q, q0 + r * a.qh + blk * 32, a.q_half, a.ocp, &packed);
+                    const int sw = C::KROW == 32 ? (r >> 2) & 1 : C::KROW == 64 ? (r >> 1) & 3 : r & 7;
+                    *reinterpret_cast<uint4*>(smem + C::OFF_Q + wg * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16)) = packed;
+                    smem[C::OFF_QSF + (wg * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb);
+                }
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(&q_full[wg]);
+                if (row == 127 && t.tile == 0 && t.hg == 0) {
+                    const int len = __ldg(a.seq_lens + t.b);
+                    if (len != t.len) record_index_error(kIndexLength, len);
+                }
             }
             bool out_of_time = false;
             // Step i: P, then the O^T of step i - 1 is added (the last has no P).
@@ -815,7 +791,6 @@ __global__ void __launch_bounds__(384, 1)
                 if ((lane & 7) == 0) red[wq * HC + 4 * c + (lane >> 3)] = sum;
             }
             ptx::named_bar_sync(bar_id, 128);
-            const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
             const bool begun = t.tile == 0;  // the item's first tile is in the range
             const bool whole = begun && t.n == t.tiles;
             const int slot = 2 * blockIdx.x + (t.left < count ? 1 : 0);
