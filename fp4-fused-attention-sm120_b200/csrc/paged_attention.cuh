@@ -27,9 +27,9 @@
 // and paged_join_kernel joins them, in order, so results repeat bit for bit.
 //
 // Roles (384 threads):
-//   warp 0      key producer (one thread): a page's codes by TMA, its raw
-//               scales by a bulk copy, into a ring of stages.
-//   warp 1      value producer (one thread): a page's V by TMA.
+//   warp 0      key producer: a page's codes by TMA, its raw scales by a bulk
+//               copy, into a ring of stages.
+//   warp 1      value producer: a page's V by TMA.
 //   warp 2      S^T issuer: brings the scales into the tensor core's layout,
 //               then one thread issues the MMAs.
 //   warp 3      O^T issuer (one thread).
@@ -406,59 +406,57 @@ __global__ void __launch_bounds__(384, 1)
     if (warp <= 1) {
         // ------------------------------------------------------------ producers
         const bool keys_role = warp == 0;
-        if (ptx::elect_one()) {
-            Ring<C::STAGES> ring;
-            int g = 0;
-            bool ok = true;
-            for (; ok && t.left > 0; t.next(a)) {
-                const int head = t.hg / a.splits;
-                const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift);
-                int id[8];  // the tile's pages (those of the next are loaded a tile ahead)
-                auto load_ids = [&](int i, int (&to)[8]) {
-                    const int keys = i < t.n ? t.keys(i) : 0;
-                    const int32_t* from = row + ((i * kPagedTile) >> shift);
+        Ring<C::STAGES> ring;
+        int g = 0;
+        bool ok = true;
+        for (; ok && t.left > 0; t.next(a)) {
+            const int head = t.hg / a.splits;
+            const uint8_t* scales = a.c.k_scales + static_cast<int64_t>(head) * page * C::NB;
+            const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift) + lane;
+            const int step = kPagedTile >> shift;  // pages of a tile; lane p has the p-th
+            int left = lane < step ? (t.len - t.tile * kPagedTile + page - 1) >> shift : 0;  // pages from this tile on
+            int id = lane < left ? __ldg(row) : 0;
+            for (int i = 0; i < t.n; i++, g++, ring.next()) {
+                row += step;
+                left -= step;
+                const int next_id = i + 1 < t.n && lane < left ? __ldg(row) : 0;
+                if (id < 0 || id >= a.c.pages) {
+                    record_index_error(kIndexPage, id);
+                    id = 0;
+                }
+                int pid[8];
 #pragma unroll
-                    for (int p = 0; p < 8; p++) to[p] = (p << shift) < keys ? __ldg(from + p) : 0;
-                };
-                load_ids(0, id);
-                for (int i = 0; i < t.n; i++, g++, ring.next()) {
-                    int next[8];
-                    load_ids(i + 1, next);
-                    const int n = (t.keys(i) + page - 1) >> shift;
-#pragma unroll
-                    for (int p = 0; p < 8; p++)
-                        if (static_cast<unsigned>(id[p]) >= static_cast<unsigned>(a.c.pages)) {
-                            record_index_error(kIndexPage, id[p]);
-                            id[p] = 0;
-                        }
-                    uint8_t* st = stages + ring.s * C::STAGE;
-                    if (g >= C::STAGES && !bounded_wait(&empty[ring.s], ring.parity ^ 1u, w, kPagedEmpty)) {
-                        ok = false;
-                        break;
-                    }
+                for (int p = 0; p < 8; p++) pid[p] = __shfl_sync(~0u, id, p);
+                const int n = (t.keys(i) + page - 1) >> shift;
+                uint8_t* st = stages + ring.s * C::STAGE;
+                if (g >= C::STAGES && !__all_sync(~0u, bounded_wait(&empty[ring.s], ring.parity ^ 1u, w, kPagedEmpty))) {
+                    ok = false;
+                    break;
+                }
+                if (ptx::elect_one()) {
                     if (keys_role) {
                         ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * (C::KROW + C::NB));
-                        const uint8_t* scales = a.c.k_scales + static_cast<int64_t>(head) * page * C::NB;
                         each_page(n, [&](int p) {
-                            ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, id[p]);
-                            ptx::bulk_load(st + C::K_BYTES + C::V_BYTES + p * page * C::NB, scales + id[p] * a.c.k_scales_stride,
+                            ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, pid[p]);
+                            ptx::bulk_load(st + C::K_BYTES + C::V_BYTES + p * page * C::NB, scales + pid[p] * a.c.k_scales_stride,
                                            page * C::NB, &k_full[ring.s]);
                         });
                     } else {
                         ptx::mbar_arrive_expect_tx(&v_full[ring.s], n * page * D * 2);
                         each_page(n, [&](int p) {
-                            ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, id[p]);
+                            ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, pid[p]);
                         });
                     }
-#pragma unroll
-                    for (int p = 0; p < 8; p++) id[p] = next[p];
                 }
+                __syncwarp();
+                id = next_id;
             }
-            // Every copy issued lands before the block exits.
+        }
+        // Every copy issued lands before the block exits.
+        if (lane == 0)
             for (int i = max(0, g - C::STAGES); i < g; i++)
                 bounded_drain(keys_role ? &k_full[i % C::STAGES] : &v_full[i % C::STAGES],
                               static_cast<uint32_t>(i / C::STAGES) & 1u, 2 * a.timeout_ns);
-        }
         __syncwarp();
     } else if (warp == 2) {
         // ------------------------------------------------------------ S^T issuer
