@@ -13,6 +13,7 @@
 #include <cstring>
 #include <mutex>
 #include <new>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -123,6 +124,20 @@ int check_rotary(const float* table, int rotary_dim, int64_t max_positions, int 
         return fail(FP4ATTN_EINVAL, "rotary_dim %d must be even, in [2, head_dim %d]", rotary_dim, head_dim);
     if (max_positions < 1) return fail(FP4ATTN_EINVAL, "max_positions must be >= 1");
     return FP4ATTN_OK;
+}
+
+// f(std::integral_constant<int, head_dim>) for a supported head_dim.
+template <typename F>
+void with_dim(int d, F f)
+{
+    switch (d) {
+        case 32: f(std::integral_constant<int, 32>{}); break;
+        case 64: f(std::integral_constant<int, 64>{}); break;
+        case 96: f(std::integral_constant<int, 96>{}); break;
+        case 128: f(std::integral_constant<int, 128>{}); break;
+        case 160: f(std::integral_constant<int, 160>{}); break;
+        default: f(std::integral_constant<int, 256>{}); break;
+    }
 }
 
 // Whether rows at these strides take 16-byte accesses.
@@ -343,7 +358,8 @@ int fp4attn_rotary(const void* x, void* y, int dtype, int batch, int heads, int 
     const int64_t turned = vec ? (interleaved ? rotary_dim / 8 : rotary_dim / 16) : rotary_dim / 2;
     const int64_t work = seq * (turned + (head_dim - rotary_dim) / (vec ? 8 : 1));
     if (work > 0x7FFFFF00) return fail(FP4ATTN_EINVAL, "seq %d is too long", seq);
-    while (a.heads_per_thread < 8 && work * batch * (heads / (2 * a.heads_per_thread)) >= 148 * 2048) a.heads_per_thread *= 2;
+    // Several heads a thread where that leaves every SM its 2048 threads.
+    while (a.heads_per_thread < 4 && work * batch * (heads / (2 * a.heads_per_thread)) >= 148 * 2048) a.heads_per_thread *= 2;
     const dim3 grid(static_cast<unsigned>((work + 255) / 256), (heads + a.heads_per_thread - 1) / a.heads_per_thread, batch);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == FP4ATTN_F16) launch_rotary<__half>(grid, st, a, vec, interleaved != 0);
@@ -394,12 +410,25 @@ int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* 
     a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
     a.vec = whole_eights(a.rot, a.interleaved) && wide(K, dtype, {a.kt, a.kh}) && wide(V, dtype, {a.vt, a.vh}) &&
             (!Q || wide(Q, dtype, {a.qt, a.qh}));
-    const int64_t units = static_cast<int64_t>(tokens) * (2 * a.c.kv_heads + a.q_heads) * (a.c.head_dim / 8);
-    if ((units + 255) / 256 > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "%d tokens are too many", tokens);
-    const unsigned grid = static_cast<unsigned>((units + 255) / 256);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FP4ATTN_F16) cache_append_kernel<__half><<<grid, 256, 0, st>>>(a);
-    else cache_append_kernel<float><<<grid, 256, 0, st>>>(a);
+    const bool f16 = dtype == FP4ATTN_F16;
+    if (a.vec && (a.interleaved || a.rot % 64 == 0)) {
+        // Heads a block takes at once, and blocks per token: one where the tokens
+        // alone fill the SMs, else one per set of heads.
+        const int units = a.interleaved ? a.c.head_dim / 8 : a.rot / 16 + (a.c.head_dim - a.rot) / 8;
+        const int at_once = kAppendThreads / units, sets = (2 * a.c.kv_heads + a.q_heads + at_once - 1) / at_once;
+        const dim3 grid(tokens, tokens >= 148 * 16 ? 1 : std::min(sets, 65535));
+        if (f16 && a.interleaved) cache_append_kernel<__half, true><<<grid, kAppendThreads, 0, st>>>(a);
+        else if (f16) cache_append_kernel<__half, false><<<grid, kAppendThreads, 0, st>>>(a);
+        else if (a.interleaved) cache_append_kernel<float, true><<<grid, kAppendThreads, 0, st>>>(a);
+        else cache_append_kernel<float, false><<<grid, kAppendThreads, 0, st>>>(a);
+    } else {
+        const int64_t work = static_cast<int64_t>(tokens) * (2 * a.c.kv_heads + a.q_heads) * (a.c.head_dim / 8);
+        if ((work + 255) / 256 > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "%d tokens are too many", tokens);
+        const unsigned grid = static_cast<unsigned>((work + 255) / 256);
+        if (f16) cache_append_any_kernel<__half><<<grid, 256, 0, st>>>(a);
+        else cache_append_any_kernel<float><<<grid, 256, 0, st>>>(a);
+    }
     PAGED_CUDA(cudaGetLastError());
     return FP4ATTN_OK;
 }
@@ -421,11 +450,11 @@ int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table,
     if (int rc = host::ready()) return rc;
     const GatherArgs a{view_of(*cache), TableView{block_table, table_stride, seqs, max_pages}, starts, lengths,
                        max_length, heads / cache->kv_heads, K, V};
-    const int64_t units = static_cast<int64_t>(max_length) * (cache->head_dim / 8);
-    const dim3 grid(static_cast<unsigned>((units + 255) / 256), cache->kv_heads, seqs);
+    const int rows = 256 / (cache->head_dim / 8) * kGatherRows;
+    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(max_length) + rows - 1) / rows), cache->kv_heads, seqs);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FP4ATTN_F16) cache_gather_kernel<__half><<<grid, 256, 0, st>>>(a);
-    else cache_gather_kernel<float><<<grid, 256, 0, st>>>(a);
+    if (dtype == FP4ATTN_F16) with_dim(cache->head_dim, [&](auto d) { cache_gather_kernel<__half, d.value><<<grid, 256, 0, st>>>(a); });
+    else with_dim(cache->head_dim, [&](auto d) { cache_gather_kernel<float, d.value><<<grid, 256, 0, st>>>(a); });
     PAGED_CUDA(cudaGetLastError());
     return FP4ATTN_OK;
 }

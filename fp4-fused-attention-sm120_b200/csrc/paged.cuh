@@ -103,38 +103,124 @@ struct AppendArgs {
     int vec;                           // 16-byte loads and whole eights in the rotary layout
 };
 
-// Eight elements e0 .. e0 + 7 of a row, rotated (FP32, not yet rounded).
+// Quantises eight elements of a key (as a separate rotation would have left
+// them) that share a block of 32 with those of the three neighbouring lanes,
+// and stores their codes and the block's scale.  `place`: the head's token in
+// its page.
 template <typename T>
-__device__ __forceinline__ void rotated8(const T* row, int e0, const float2* cs, int rot, int interleaved, int vec,
-                                         float (&v)[8])
+__device__ __forceinline__ void put_key(const CacheView& c, int page, int64_t place, int e0, float (&v)[8], int ocp)
+{
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        v[i] = to_float(from_float<T>(v[i]));
+        amax = fmaxf(amax, fabsf(v[i]));
+    }
+    const uint32_t quad = 0xFu << ((threadIdx.x & 31) & ~3);
+    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+    const uint32_t sb = scale_byte(amax, ocp);
+    *reinterpret_cast<uint32_t*>(c.k_codes + page * c.k_codes_stride + place * (c.head_dim / 2) + e0 / 2) = encode8<T>(v, sb);
+    if (e0 % 32 == 0)
+        c.k_scales[page * c.k_scales_stride + place * (c.head_dim / 32) + e0 / 32] = static_cast<uint8_t>(sb == 255u ? 254u : sb);
+}
+
+// One block per token (and, with few tokens, per set of its heads).  A thread
+// has eight elements of a row and (halves) the eight they are paired with, or
+// eight interleaved ones, or eight that are not turned; its cosines and sines
+// are loaded once and serve every head it walks.  Bound by memory: a token's
+// K, V and Q in, Q out, 17/32 + 2 bytes an element into the cache.  Needs
+// 16-byte aligned rows and, for halves, a rotary dimension of whole 64s, so
+// that a block of 32 is four neighbouring lanes'.
+constexpr int kAppendThreads = 128;
+
+template <typename T, bool kInter>
+__global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const __grid_constant__ AppendArgs a)
+{
+    const int D = a.c.head_dim, half = a.rot / 2, pairs = kInter ? 0 : half / 8;
+    const int units = kInter ? D / 8 : pairs + (D - a.rot) / 8, at_once = kAppendThreads / units;
+    const int hs = threadIdx.x / units, u = threadIdx.x % units;
+    if (hs >= at_once) return;
+    const bool pair = !kInter && u < pairs;
+    const int e0 = kInter || pair ? 8 * u : a.rot + 8 * (u - pairs);
+    const int tok = blockIdx.x, kv = a.c.kv_heads, heads = 2 * kv + a.q_heads;  // K, V, Q
+    const int pos = __ldg(a.positions + tok);
+    const bool valid = pos >= 0 && (!a.rot || pos < a.max_positions);
+    if (pos >= 0 && !valid && threadIdx.x == 0 && blockIdx.y == 0) record_index_error(kIndexPosition, pos);
+    int page = -1;
+    if (valid && static_cast<int>(blockIdx.y) * at_once < 2 * kv) page = page_of(a.c, a.t, a.seq_ids ? __ldg(a.seq_ids + tok) : tok, pos);
+    constexpr int P = kInter ? 4 : 8;
+    float2 cs[P];
+    if (valid && (pair || (kInter && e0 < a.rot))) {
+        const float4* f = reinterpret_cast<const float4*>(a.table + static_cast<int64_t>(pos) * half + (kInter ? e0 / 2 : e0));
+#pragma unroll
+        for (int i = 0; i < P / 2; i++) {
+            const float4 g = __ldg(f + i);
+            cs[2 * i] = make_float2(g.x, g.y);
+            cs[2 * i + 1] = make_float2(g.z, g.w);
+        }
+    }
+    const int64_t in_page = pos & (a.c.page_size - 1);
+#pragma unroll 1
+    for (int h = blockIdx.y * at_once + hs; h < heads; h += at_once * gridDim.y) {
+        if (h >= kv && h < 2 * kv) {
+            if (page < 0) continue;
+            const T* x = static_cast<const T*>(a.v) + tok * a.vt + (h - kv) * a.vh + e0;
+            __half* dst = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.c.v) + page * a.c.v_stride) +
+                          ((h - kv) * a.c.page_size + in_page) * D + e0;
+            if constexpr (sizeof(T) == 2) {  // FP16 values keep their bits
+                const uint4 va = *reinterpret_cast<const uint4*>(x);
+                if (pair) *reinterpret_cast<uint4*>(dst + half) = *reinterpret_cast<const uint4*>(x + half);
+                *reinterpret_cast<uint4*>(dst) = va;
+            } else {
+                float v[8];
+                load8v(x, v);
+                store8v(dst, v);
+                if (pair) {
+                    load8v(x + half, v);
+                    store8v(dst + half, v);
+                }
+            }
+            continue;
+        }
+        const bool is_q = h >= 2 * kv;
+        if (!is_q && page < 0) continue;
+        const T* x = is_q ? static_cast<const T*>(a.q) + tok * a.qt + (h - 2 * kv) * a.qh
+                          : static_cast<const T*>(a.k) + tok * a.kt + h * a.kh;
+        float v[8], w[8];
+        load8v(x + e0, v);
+        if (pair) {
+            load8v(x + e0 + half, w);
+            if (valid) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) turn(v[i], w[i], cs[i % P].x, cs[i % P].y, v[i], w[i]);
+            }
+        } else if (kInter && e0 < a.rot && valid) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) turn(v[2 * i], v[2 * i + 1], cs[i].x, cs[i].y, v[2 * i], v[2 * i + 1]);
+        }
+        if (is_q) {
+            if (!valid) {  // padding, and angles that are not there: a row of zeros
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = w[i] = 0.f;
+            }
+            T* dst = static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + h - 2 * kv) * D + e0;
+            store8v(dst, v);
+            if (pair) store8v(dst + half, w);
+        } else {
+            const int64_t place = static_cast<int64_t>(h) * a.c.page_size + in_page;
+            put_key<T>(a.c, page, place, e0, v, a.ocp);
+            if (pair) put_key<T>(a.c, page, place, e0 + half, w, a.ocp);
+        }
+    }
+}
+
+// Eight elements e0 .. e0 + 7 of a row, rotated one by one (FP32, not yet
+// rounded).
+template <typename T>
+__device__ __forceinline__ void rotated8(const T* row, int e0, const float2* cs, int rot, int interleaved, float (&v)[8])
 {
     const int half = rot / 2;
-    if (vec) {
-        load8v(row + e0, v);
-        if (e0 >= rot) return;
-        if (interleaved) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = __ldg(cs + e0 / 2 + i);
-                turn(v[2 * i], v[2 * i + 1], f.x, f.y, v[2 * i], v[2 * i + 1]);
-            }
-        } else {
-            const bool first = e0 < half;
-            float w[8];
-            load8v(row + (first ? e0 + half : e0 - half), w);
-            const float2* f8 = cs + (first ? e0 : e0 - half);
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(f8 + i));
-                float ra, rb;
-                turn(first ? v[i] : w[i], first ? w[i] : v[i], f.x, f.y, ra, rb);
-                v[i] = first ? ra : rb;
-                turn(first ? v[i + 1] : w[i + 1], first ? w[i + 1] : v[i + 1], f.z, f.w, ra, rb);
-                v[i + 1] = first ? ra : rb;
-            }
-        }
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int e = e0 + i;
@@ -150,13 +236,14 @@ __device__ __forceinline__ void rotated8(const T* row, int e0, const float2* cs,
     }
 }
 
-// One thread per eight elements of a token's K, V or Q; four neighbouring
-// lanes share a block of 32 and its scale.
+// Any alignment, stride and rotary dimension: one thread per eight elements of
+// a token's K, V or Q, four neighbouring lanes to a block of 32, every element
+// loaded by itself.
 template <typename T>
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a)
+__global__ void __launch_bounds__(256) cache_append_any_kernel(const __grid_constant__ AppendArgs a)
 {
     const int D = a.c.head_dim, row8 = D / 8;
-    const int kv_units = a.c.kv_heads * row8, units = 2 * kv_units + (a.q ? a.q_heads * row8 : 0);
+    const int kv_units = a.c.kv_heads * row8, units = 2 * kv_units + a.q_heads * row8;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (n >= static_cast<int64_t>(a.tokens) * units) return;
     const int tok = static_cast<int>(n / units);
@@ -166,66 +253,35 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a)
     const bool is_v = !is_q && u >= kv_units;
     u -= is_q ? 2 * kv_units : is_v ? kv_units : 0;
     const int head = u / row8, e0 = (u % row8) * 8;
-    if (pos < 0) {  // padding: nothing enters the cache, the query row is zero
-        if (is_q) {
-            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            store8v(static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + head) * D + e0, z);
-        }
-        return;
-    }
-    const bool angle_ok = !a.table || pos < a.max_positions;
-    if (!angle_ok) record_index_error(kIndexPosition, pos);
-    const float2* cs = a.table ? a.table + (angle_ok ? pos : 0) * static_cast<int64_t>(a.rot / 2) : nullptr;
+    const bool valid = pos >= 0 && (!a.rot || pos < a.max_positions);
+    if (pos >= 0 && !valid) record_index_error(kIndexPosition, pos);
+    const float2* cs = a.rot ? a.table + (valid ? pos : 0) * static_cast<int64_t>(a.rot / 2) : nullptr;
     float v[8];
     if (is_q) {
-        if (!angle_ok) {
+        rotated8(static_cast<const T*>(a.q) + tok * a.qt + head * a.qh, e0, cs, a.rot, a.interleaved, v);
+        if (!valid) {  // padding, and angles that are not there: a row of zeros
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = 0.f;
-        } else
-            rotated8(static_cast<const T*>(a.q) + tok * a.qt + head * a.qh, e0, cs, a.rot, a.interleaved, a.vec, v);
+        }
         store8v(static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + head) * D + e0, v);
         return;
     }
+    if (!valid) return;
     const int page = page_of(a.c, a.t, a.seq_ids ? a.seq_ids[tok] : tok, pos);
-    if (page < 0 || !angle_ok) return;
-    const int64_t in_page = static_cast<int64_t>(head) * a.c.page_size + (pos & (a.c.page_size - 1));
+    if (page < 0) return;
+    const int64_t place = static_cast<int64_t>(head) * a.c.page_size + (pos & (a.c.page_size - 1));
     if (is_v) {
         const T* row = static_cast<const T*>(a.v) + tok * a.vt + head * a.vh + e0;
-        __half* dst = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.c.v) + page * a.c.v_stride) + in_page * D + e0;
-        if constexpr (sizeof(T) == 2) {  // FP16 values keep their bits
-            if (a.vec) {
-                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(row);
-            } else {
+        __half* dst = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.c.v) + page * a.c.v_stride) + place * D + e0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) dst[i] = row[i];
-            }
-        } else {
-            if (a.vec) {
-                load8v(row, v);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = row[i];
-            }
-            store8v(dst, v);
+        for (int i = 0; i < 8; i++) {
+            if constexpr (sizeof(T) == 2) dst[i] = row[i];
+            else dst[i] = __float2half_rn(row[i]);
         }
         return;
     }
-    rotated8(static_cast<const T*>(a.k) + tok * a.kt + head * a.kh, e0, cs, a.rot, a.interleaved, a.vec, v);
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        v[i] = to_float(from_float<T>(v[i]));  // the key as a separate rotation would have left it
-        amax = fmaxf(amax, fabsf(v[i]));
-    }
-    const uint32_t quad = 0xFu << ((threadIdx.x & 31) & ~3);
-    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
-    const uint32_t sb = scale_byte(amax, a.ocp);
-    const uint32_t w = encode8<T>(v, sb);
-    *reinterpret_cast<uint32_t*>(a.c.k_codes + page * a.c.k_codes_stride + in_page * (D / 2) + e0 / 2) = w;
-    if ((u & 3) == 0)
-        a.c.k_scales[page * a.c.k_scales_stride + in_page * (D / 32) + e0 / 32] =
-            static_cast<uint8_t>(sb == 255u ? 254u : sb);
+    rotated8(static_cast<const T*>(a.k) + tok * a.kt + head * a.kh, e0, cs, a.rot, a.interleaved, v);
+    put_key<T>(a.c, page, place, e0, v, a.ocp);
 }
 
 // Exactly 2^(sb - 127).
@@ -250,38 +306,66 @@ struct GatherArgs {
     void *k, *v;                      // [seqs][kv_heads * repeat][max_length][head_dim]
 };
 
-// One thread per eight elements of a token's K and V of one head; rows past a
-// sequence's length are written as zeros.
-template <typename T>
-__global__ void __launch_bounds__(256) cache_gather_kernel(const GatherArgs a)
+// Thread: eight elements of the K and V of kGatherRows tokens of one head, the
+// block's rows apart, all of them loaded before the first is stored.  Rows past
+// a sequence's length are written as zeros.
+constexpr int kGatherRows = 4;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) cache_gather_kernel(const __grid_constant__ GatherArgs a)
 {
-    const int D = a.c.head_dim, row8 = D / 8;
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (n >= static_cast<int64_t>(a.max_length) * row8) return;
+    constexpr int ROW8 = D / 8, ROWS = 256 / ROW8;  // rows of a block at once
+    const int tid = threadIdx.x, e0 = tid % ROW8 * 8, r = tid / ROW8;
+    if (r >= ROWS) return;
     const int head = blockIdx.y, seq = blockIdx.z;
-    const int i = static_cast<int>(n / row8), e0 = static_cast<int>(n % row8) * 8;
-    float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const int start = a.starts ? a.starts[seq] : 0, length = a.lengths[seq];
+    const int start = a.starts ? __ldg(a.starts + seq) : 0;
+    int length = __ldg(a.lengths + seq);
     if (start < 0 || length < 0 || length > a.max_length) {
-        if (n == 0 && head == 0) record_index_error(kIndexLength, start < 0 ? start : length);
-    } else if (i < length) {
-        const int64_t pos = static_cast<int64_t>(start) + i;
-        const int page = pos > 0x7FFFFFFF ? -1 : page_of(a.c, a.t, seq, static_cast<int>(pos));
-        if (page >= 0) {
-            const int64_t in_page = static_cast<int64_t>(head) * a.c.page_size + (pos & (a.c.page_size - 1));
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(a.c.k_codes + page * a.c.k_codes_stride +
-                                                                  in_page * (D / 2) + e0 / 2);
-            const float sc = scale_value(a.c.k_scales[page * a.c.k_scales_stride + in_page * (D / 32) + e0 / 32]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) k[j] = e2m1_value((w >> (4 * j)) & 15u) * sc;
-            load8v(reinterpret_cast<const __half*>(reinterpret_cast<const uint8_t*>(a.c.v) + page * a.c.v_stride) +
-                       in_page * D + e0, v);
-        }
+        if (blockIdx.x == 0 && head == 0 && tid == 0) record_index_error(kIndexLength, start < 0 ? start : length);
+        length = 0;
     }
-    for (int r = 0; r < a.repeat; r++) {
-        const int64_t at = ((static_cast<int64_t>(seq) * a.c.kv_heads + head) * a.repeat + r) * a.max_length + i;
-        store8v(static_cast<T*>(a.k) + at * D + e0, k);
-        store8v(static_cast<T*>(a.v) + at * D + e0, v);
+    uint32_t code[kGatherRows];
+    float scale[kGatherRows];
+    uint4 value[kGatherRows];
+#pragma unroll
+    for (int k = 0; k < kGatherRows; k++) {
+        const int i = (blockIdx.x * kGatherRows + k) * ROWS + r;
+        code[k] = 0u;
+        scale[k] = 0.f;
+        value[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (i >= length) continue;
+        const int64_t pos = static_cast<int64_t>(start) + i;
+        if (pos > 0x7FFFFFFF) {
+            record_index_error(kIndexLength, pos);
+            continue;
+        }
+        const int page = page_of(a.c, a.t, seq, static_cast<int>(pos));
+        if (page < 0) continue;
+        const int64_t in_page = static_cast<int64_t>(head) * a.c.page_size + (pos & (a.c.page_size - 1));
+        code[k] = __ldg(reinterpret_cast<const uint32_t*>(a.c.k_codes + page * a.c.k_codes_stride + in_page * (D / 2) + e0 / 2));
+        scale[k] = scale_value(__ldg(a.c.k_scales + page * a.c.k_scales_stride + in_page * (D / 32) + e0 / 32));
+        value[k] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.c.v) + page * a.c.v_stride +
+                                                        (in_page * D + e0) * 2));
+    }
+#pragma unroll
+    for (int k = 0; k < kGatherRows; k++) {
+        const int i = (blockIdx.x * kGatherRows + k) * ROWS + r;
+        if (i >= a.max_length) return;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = e2m1_value((code[k] >> (4 * j)) & 15u) * scale[k];
+        for (int q = 0; q < a.repeat; q++) {
+            const int64_t at = ((static_cast<int64_t>(seq) * a.c.kv_heads + head) * a.repeat + q) * a.max_length + i;
+            store8v(static_cast<T*>(a.k) + at * D + e0, x);
+            T* v = static_cast<T*>(a.v) + at * D + e0;
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<uint4*>(v) = value[k];
+            } else {
+                float f[8];
+                load8v(reinterpret_cast<const __half*>(&value[k]), f);
+                store8v(v, f);
+            }
+        }
     }
 }
 
