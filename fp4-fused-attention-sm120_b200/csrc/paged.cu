@@ -413,11 +413,10 @@ int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = dtype == FP4ATTN_F16;
     if (a.vec && (a.interleaved || a.rot % 64 == 0)) {
-        // Heads a block takes at once, and blocks per token: one where the tokens
-        // alone fill the SMs, else one per set of heads.
         const int units = a.interleaved ? a.c.head_dim / 8 : a.rot / 16 + (a.c.head_dim - a.rot) / 8;
         const int at_once = kAppendThreads / units, sets = (2 * a.c.kv_heads + a.q_heads + at_once - 1) / at_once;
-        const dim3 grid(tokens, tokens >= 148 * 16 ? 1 : std::min(sets, 65535));
+        if (sets > 65535) return fail(FP4ATTN_EINVAL, "%d heads are too many", 2 * a.c.kv_heads + a.q_heads);
+        const dim3 grid(tokens, sets);
         if (f16 && a.interleaved) cache_append_kernel<__half, true><<<grid, kAppendThreads, 0, st>>>(a);
         else if (f16) cache_append_kernel<__half, false><<<grid, kAppendThreads, 0, st>>>(a);
         else if (a.interleaved) cache_append_kernel<float, true><<<grid, kAppendThreads, 0, st>>>(a);

@@ -125,93 +125,94 @@ __device__ __forceinline__ void put_key(const CacheView& c, int page, int64_t pl
         c.k_scales[page * c.k_scales_stride + place * (c.head_dim / 32) + e0 / 32] = static_cast<uint8_t>(sb == 255u ? 254u : sb);
 }
 
-// One block per token (and, with few tokens, per set of its heads).  A thread
-// has eight elements of a row and (halves) the eight they are paired with, or
-// eight interleaved ones, or eight that are not turned; its cosines and sines
-// are loaded once and serve every head it walks.  Bound by memory: a token's
-// K, V and Q in, Q out, 17/32 + 2 bytes an element into the cache.  Needs
-// 16-byte aligned rows and, for halves, a rotary dimension of whole 64s, so
-// that a block of 32 is four neighbouring lanes'.
+// Eight elements as they lie in memory, and as floats.
+__device__ __forceinline__ void load_raw8(const __half* p, uint4 (&r)[1]) { r[0] = *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void load_raw8(const float* p, uint4 (&r)[2])
+{
+    r[0] = reinterpret_cast<const uint4*>(p)[0];
+    r[1] = reinterpret_cast<const uint4*>(p)[1];
+}
+
+// A block has one token and a set of its heads.  A thread has eight elements
+// of a row and (halves) the eight they are paired with, or eight interleaved
+// ones, or eight that are not turned.  Bound by memory: a token's K, V and Q
+// in, Q out, 17/32 + 2 bytes an element into the cache.  What there is to wait
+// for -- the position, then the angles and the page -- is waited for while the
+// row is on its way, once: a thread that walked three heads with its angles
+// kept, and 16 of its 78 registers for them, took 156 us for 17,600 tokens of 32 + 2 x 8
+// heads of 128.  Needs 16-byte aligned rows and, for halves, a rotary dimension
+// of whole 64s, so that a block of 32 is four neighbouring lanes'.
 constexpr int kAppendThreads = 128;
 
 template <typename T, bool kInter>
-__global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const __grid_constant__ AppendArgs a)
+__global__ void __launch_bounds__(kAppendThreads, 8) cache_append_kernel(const __grid_constant__ AppendArgs a)
 {
     const int D = a.c.head_dim, half = a.rot / 2, pairs = kInter ? 0 : half / 8;
     const int units = kInter ? D / 8 : pairs + (D - a.rot) / 8, at_once = kAppendThreads / units;
     const int hs = threadIdx.x / units, u = threadIdx.x % units;
-    if (hs >= at_once) return;
-    const bool pair = !kInter && u < pairs;
+    const int tok = blockIdx.x, kv = a.c.kv_heads, h = blockIdx.y * at_once + hs;  // K, V, Q
+    if (hs >= at_once || h >= 2 * kv + a.q_heads) return;
+    const bool pair = !kInter && u < pairs, is_v = h >= kv && h < 2 * kv, is_q = h >= 2 * kv;
     const int e0 = kInter || pair ? 8 * u : a.rot + 8 * (u - pairs);
-    const int tok = blockIdx.x, kv = a.c.kv_heads, heads = 2 * kv + a.q_heads;  // K, V, Q
+    const T* x = (is_q   ? static_cast<const T*>(a.q) + tok * a.qt + (h - 2 * kv) * a.qh
+                  : is_v ? static_cast<const T*>(a.v) + tok * a.vt + (h - kv) * a.vh
+                         : static_cast<const T*>(a.k) + tok * a.kt + h * a.kh) + e0;
+    uint4 ra[sizeof(T) / 2], rb[sizeof(T) / 2];
+    load_raw8(x, ra);
+    if (pair) load_raw8(x + half, rb);
     const int pos = __ldg(a.positions + tok);
     const bool valid = pos >= 0 && (!a.rot || pos < a.max_positions);
-    if (pos >= 0 && !valid && threadIdx.x == 0 && blockIdx.y == 0) record_index_error(kIndexPosition, pos);
     int page = -1;
-    if (valid && static_cast<int>(blockIdx.y) * at_once < 2 * kv) page = page_of(a.c, a.t, a.seq_ids ? __ldg(a.seq_ids + tok) : tok, pos);
-    constexpr int P = kInter ? 4 : 8;
-    float2 cs[P];
-    if (valid && (pair || (kInter && e0 < a.rot))) {
-        const float4* f = reinterpret_cast<const float4*>(a.table + static_cast<int64_t>(pos) * half + (kInter ? e0 / 2 : e0));
+    if (valid && !is_q) page = page_of(a.c, a.t, a.seq_ids ? __ldg(a.seq_ids + tok) : tok, pos);
+    if (!valid && pos >= 0 && u == 0 && h == 0) record_index_error(kIndexPosition, pos);
+    if (!is_q && page < 0) return;
+    const int64_t place = static_cast<int64_t>(is_v ? h - kv : h) * a.c.page_size + (pos & (a.c.page_size - 1));
+    if (is_v) {
+        __half* dst = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.c.v) + page * a.c.v_stride) + place * D + e0;
+        if constexpr (sizeof(T) == 2) {  // FP16 values keep their bits
+            *reinterpret_cast<uint4*>(dst) = ra[0];
+            if (pair) *reinterpret_cast<uint4*>(dst + half) = rb[0];
+        } else {
+            float v[8];
+            load8v(reinterpret_cast<const T*>(ra), v);
+            store8v(dst, v);
+            if (pair) {
+                load8v(reinterpret_cast<const T*>(rb), v);
+                store8v(dst + half, v);
+            }
+        }
+        return;
+    }
+    float v[8], w[8];
+    load8v(reinterpret_cast<const T*>(ra), v);
+    if (pair) load8v(reinterpret_cast<const T*>(rb), w);
+    if (!valid) {  // padding, and angles that are not there: a row of zeros
 #pragma unroll
-        for (int i = 0; i < P / 2; i++) {
-            const float4 g = __ldg(f + i);
-            cs[2 * i] = make_float2(g.x, g.y);
-            cs[2 * i + 1] = make_float2(g.z, g.w);
+        for (int i = 0; i < 8; i++) v[i] = w[i] = 0.f;
+    } else if (pair) {
+        const float4* cs = reinterpret_cast<const float4*>(a.table + static_cast<int64_t>(pos) * half + e0);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 f = __ldg(cs + i);
+            turn(v[2 * i], w[2 * i], f.x, f.y, v[2 * i], w[2 * i]);
+            turn(v[2 * i + 1], w[2 * i + 1], f.z, f.w, v[2 * i + 1], w[2 * i + 1]);
+        }
+    } else if (kInter && e0 < a.rot) {
+        const float4* cs = reinterpret_cast<const float4*>(a.table + static_cast<int64_t>(pos) * half + e0 / 2);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float4 f = __ldg(cs + i);
+            turn(v[4 * i], v[4 * i + 1], f.x, f.y, v[4 * i], v[4 * i + 1]);
+            turn(v[4 * i + 2], v[4 * i + 3], f.z, f.w, v[4 * i + 2], v[4 * i + 3]);
         }
     }
-    const int64_t in_page = pos & (a.c.page_size - 1);
-#pragma unroll 1
-    for (int h = blockIdx.y * at_once + hs; h < heads; h += at_once * gridDim.y) {
-        if (h >= kv && h < 2 * kv) {
-            if (page < 0) continue;
-            const T* x = static_cast<const T*>(a.v) + tok * a.vt + (h - kv) * a.vh + e0;
-            __half* dst = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.c.v) + page * a.c.v_stride) +
-                          ((h - kv) * a.c.page_size + in_page) * D + e0;
-            if constexpr (sizeof(T) == 2) {  // FP16 values keep their bits
-                const uint4 va = *reinterpret_cast<const uint4*>(x);
-                if (pair) *reinterpret_cast<uint4*>(dst + half) = *reinterpret_cast<const uint4*>(x + half);
-                *reinterpret_cast<uint4*>(dst) = va;
-            } else {
-                float v[8];
-                load8v(x, v);
-                store8v(dst, v);
-                if (pair) {
-                    load8v(x + half, v);
-                    store8v(dst + half, v);
-                }
-            }
-            continue;
-        }
-        const bool is_q = h >= 2 * kv;
-        if (!is_q && page < 0) continue;
-        const T* x = is_q ? static_cast<const T*>(a.q) + tok * a.qt + (h - 2 * kv) * a.qh
-                          : static_cast<const T*>(a.k) + tok * a.kt + h * a.kh;
-        float v[8], w[8];
-        load8v(x + e0, v);
-        if (pair) {
-            load8v(x + e0 + half, w);
-            if (valid) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) turn(v[i], w[i], cs[i % P].x, cs[i % P].y, v[i], w[i]);
-            }
-        } else if (kInter && e0 < a.rot && valid) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) turn(v[2 * i], v[2 * i + 1], cs[i].x, cs[i].y, v[2 * i], v[2 * i + 1]);
-        }
-        if (is_q) {
-            if (!valid) {  // padding, and angles that are not there: a row of zeros
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = w[i] = 0.f;
-            }
-            T* dst = static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + h - 2 * kv) * D + e0;
-            store8v(dst, v);
-            if (pair) store8v(dst + half, w);
-        } else {
-            const int64_t place = static_cast<int64_t>(h) * a.c.page_size + in_page;
-            put_key<T>(a.c, page, place, e0, v, a.ocp);
-            if (pair) put_key<T>(a.c, page, place, e0 + half, w, a.ocp);
-        }
+    if (is_q) {
+        T* dst = static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + h - 2 * kv) * D + e0;
+        store8v(dst, v);
+        if (pair) store8v(dst + half, w);
+    } else {
+        put_key<T>(a.c, page, place, e0, v, a.ocp);
+        if (pair) put_key<T>(a.c, page, place, e0 + half, w, a.ocp);
     }
 }
 
