@@ -138,14 +138,15 @@ __device__ __forceinline__ void load_raw8(const float* p, uint4 (&r)[2])
 // ones, or eight that are not turned.  Bound by memory: a token's K, V and Q
 // in, Q out, 17/32 + 2 bytes an element into the cache.  What there is to wait
 // for -- the position, then the angles and the page -- is waited for while the
-// row is on its way, once: a thread that walked three heads with its angles
-// kept, and 16 of its 78 registers for them, took 156 us for 17,600 tokens of 32 + 2 x 8
-// heads of 128.  Needs 16-byte aligned rows and, for halves, a rotary dimension
+// row is on its way, once, and 32 registers leave room for all the warps that an
+// SM holds: 17,600 tokens of 32 + 2 x 8 heads of 128 take 95 us, 0.67 of their
+// 63 us at the copy rate.  (With 50 registers 114 us; with three heads a thread,
+// their angles kept, and 78 registers 156.)  Needs 16-byte aligned rows and, for halves, a rotary dimension
 // of whole 64s, so that a block of 32 is four neighbouring lanes'.
 constexpr int kAppendThreads = 128;
 
 template <typename T, bool kInter>
-__global__ void __launch_bounds__(kAppendThreads, 8) cache_append_kernel(const __grid_constant__ AppendArgs a)
+__global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const __grid_constant__ AppendArgs a)
 {
     const int D = a.c.head_dim, half = a.rot / 2, pairs = kInter ? 0 : half / 8;
     const int units = kInter ? D / 8 : pairs + (D - a.rot) / 8, at_once = kAppendThreads / units;
