@@ -110,7 +110,7 @@ struct PagedCfg {
     // The O^T MMA reads 128 rows (head-dim columns) of V: past head_dim it
     // reads on into what follows; those rows of O^T are not used.
     static constexpr int V_OVER = (MT * 128 - D) / CHE * kPagedTile * CB;
-    static constexpr int MISC = 2048;                                // barriers, reductions
+    static constexpr int MISC = 3072;                                // barriers, reductions
     static constexpr int kBudget = 227 * 1024 - 1024 - OFF_STAGE - MISC - V_OVER;
     static constexpr int STAGES = kBudget / STAGE < 8 ? kBudget / STAGE : 8;
     static_assert(STAGES >= 2, "shared memory budget exceeded");
@@ -171,12 +171,13 @@ __device__ __forceinline__ int paged_block(int total, int tile, int blocks)
 // The walk over the items, or parts of items, in a block's range; every role
 // makes its own.
 struct ItemWalk {
-    int b, hg, tile, n, left;  // the part: its first tile and number of tiles; tiles left in the range, its own included
-    int len, tiles;            // the sequence's
+    int b, head, split, tile, n, left;  // the part: its first tile and number of tiles; tiles left in the range, its own included
+    int len, tiles;                     // the sequence's
     __device__ __forceinline__ void begin(const PagedArgs& a, const int4& start, int count)
     {
         b = start.x;
-        hg = start.y;
+        head = start.y / a.splits;  // (the only division: later ones would be on the way from item to item)
+        split = start.y % a.splits;
         tile = start.z;
         left = count;
         n = 0;
@@ -190,14 +191,18 @@ struct ItemWalk {
     {
         left -= n;
         tile = 0;
-        if (left > 0 && ++hg == a.head_groups) {
-            hg = 0;
-            b++;
-            len = paged_length(a, b);
-            tiles = paged_tiles(len);
+        if (left > 0 && ++split == a.splits) {
+            split = 0;
+            if (++head == a.c.kv_heads) {
+                head = 0;
+                b++;
+                len = paged_length(a, b);
+                tiles = paged_tiles(len);
+            }
         }
         n = min(left, tiles);
     }
+    __device__ __forceinline__ bool first_of_sequence() const { return tile == 0 && head == 0 && split == 0; }
     // Keys of the part's i-th tile.
     __device__ __forceinline__ int keys(int i) const { return max(0, min(kPagedTile, len - (tile + i) * kPagedTile)); }
 };
@@ -349,8 +354,8 @@ __global__ void __launch_bounds__(384, 1)
     uint64_t* o_full = p_full + 2;         // [2] O^T computed, P read (commit)
     uint64_t* o_free = o_full + 2;         // [2] O^T in registers (128)
     uint64_t* drain = o_free + 2;          // [2] everything an issuer issued is done (exit)
-    float* red_all = reinterpret_cast<float*>(smem + C::OFF_MISC + 512);  // [2][4][HC]
-    int* scratch = reinterpret_cast<int*>(smem + C::OFF_MISC + 1536);     // [8]
+    float* red_all = reinterpret_cast<float*>(smem + C::OFF_MISC + 512);  // [2 warpgroups][maxima, sums][4][HC]
+    int* scratch = reinterpret_cast<int*>(smem + C::OFF_MISC + 2560);     // [8]
     PagedRange* range = reinterpret_cast<PagedRange*>(scratch + 8);
     uint32_t* tmem_sh = reinterpret_cast<uint32_t*>(scratch + 16);
     int* abort_sh = scratch + 17;
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(384, 1)
         int g = 0;
         bool ok = true;
         for (; ok && t.left > 0; t.next(a)) {
-            const int head = t.hg / a.splits;
+            const int head = t.head;
             const uint8_t* scales = a.c.k_scales + static_cast<int64_t>(head) * page * C::NB;
             const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift) + lane;
             const int step = kPagedTile >> shift;  // pages of a tile; lane p has the p-th
@@ -596,7 +601,10 @@ __global__ void __launch_bounds__(384, 1)
         const int wg = (warp - 4) / 4, wq = warp % 4, row = wq * 32 + lane;  // key of the tile; head-dim row of O^T
         const uint32_t lanes = tmem + (static_cast<uint32_t>(wq * 32) << 16);
         const int bar_id = 1 + wg;
-        float* red = red_all + wg * 4 * HC;
+        // (A warp writes sums only after all 128 threads have read the maxima, and
+        // the other way round: an item's O^T needs the P of every thread.)
+        float* red = red_all + wg * 8 * HC;
+        float* red_sum = red + 4 * HC;
         constexpr float kGrowth = 8.f;  // how far (log2) a score may exceed the reference
         float nm[HC], l[HC], o[C::MT][HC];  // minus the reference, this thread's sums, O^T
         bool ok = true;  // no wait of this thread has run out
@@ -618,11 +626,11 @@ __global__ void __launch_bounds__(384, 1)
                 ring.parity ^= static_cast<uint32_t>(t.n / C::STAGES) & 1u;
                 continue;
             }
-            const int h0 = (t.hg % a.splits) * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
+            const int h0 = t.split * a.heads_per_group, nh = min(a.heads_per_group, a.group - h0);
             // This item's queries, while the other warpgroup has the item before.
             // (S^T of this warpgroup's last item, the buffer's last use, is computed.)
             {
-                const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(t.hg / a.splits) * a.group + h0) * a.qh;
+                const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(t.head) * a.group + h0) * a.qh;
                 for (int k = row; k < nh * C::NB; k += 128) {
                     const int r = k / C::NB, blk = k % C::NB;
                     uint4 packed;
@@ -633,7 +641,7 @@ __global__ void __launch_bounds__(384, 1)
                 }
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(&q_full[wg]);
-                if (row == 127 && t.tile == 0 && t.hg == 0) {
+                if (row == 127 && t.first_of_sequence()) {
                     const int len = __ldg(a.seq_lens + t.b);
                     if (len != t.len) record_index_error(kIndexLength, len);
                 }
@@ -656,7 +664,7 @@ __global__ void __launch_bounds__(384, 1)
                     ptx::tc_fence_before();
                     ptx::mbar_arrive(&s_free[buf]);
                     float x[C::U][HC];  // the scores, log2 domain, less the reference
-                    bool over = i == 0 || !ok;
+                    bool over = !ok;
 #pragma unroll
                     for (int u = 0; u < C::U; u++) {
                         const int keys = i * C::U + u < t.n ? t.keys(i * C::U + u) : 0;
@@ -670,13 +678,9 @@ __global__ void __launch_bounds__(384, 1)
                             over |= x[u][h] > kGrowth;
                         }
                     }
-                    if (ptx::named_bar_any(bar_id, 128, over)) {
-                        // Rare: a new item, a score that outgrew the reference, or
+                    if (i == 0 || ptx::named_bar_any(bar_id, 128, over)) {
+                        // A new item, or, rarely, a score that outgrew the reference or
                         // a wait that ran out.  All 128 threads come here together.
-                        if (ptx::named_bar_any(bar_id, 128, !ok)) {
-                            out_of_time = true;
-                            break;
-                        }
 #pragma unroll
                         for (int c = 0; c < HC / 4; c++) {
                             float v[4];
@@ -685,7 +689,10 @@ __global__ void __launch_bounds__(384, 1)
                             const float top = warp_reduce4(v, lane, max_of);
                             if ((lane & 7) == 0) red[wq * HC + 4 * c + (lane >> 3)] = top;
                         }
-                        ptx::named_bar_sync(bar_id, 128);
+                        if (ptx::named_bar_any(bar_id, 128, !ok)) {
+                            out_of_time = true;
+                            break;
+                        }
 #pragma unroll
                         for (int h = 0; h < HC; h++) {
                             const float top = fmaxf(fmaxf(red[h], red[HC + h]), fmaxf(red[2 * HC + h], red[3 * HC + h]));
@@ -786,17 +793,17 @@ __global__ void __launch_bounds__(384, 1)
             for (int c = 0; c < HC / 4; c++) {
                 const float v[4] = {l[4 * c], l[4 * c + 1], l[4 * c + 2], l[4 * c + 3]};
                 const float sum = warp_reduce4(v, lane, sum_of);
-                if ((lane & 7) == 0) red[wq * HC + 4 * c + (lane >> 3)] = sum;
+                if ((lane & 7) == 0) red_sum[wq * HC + 4 * c + (lane >> 3)] = sum;
             }
             ptx::named_bar_sync(bar_id, 128);
             const bool begun = t.tile == 0;  // the item's first tile is in the range
             const bool whole = begun && t.n == t.tiles;
             const int slot = 2 * blockIdx.x + (t.left < count ? 1 : 0);
-            const int64_t o0 = static_cast<int64_t>(t.b) * a.q_heads + (t.hg / a.splits) * a.group + h0;
+            const int64_t o0 = static_cast<int64_t>(t.b) * a.q_heads + t.head * a.group + h0;
 #pragma unroll
             for (int h = 0; h < HC; h++) {
                 if (h >= nh) break;
-                const float sum = (red[h] + red[HC + h]) + (red[2 * HC + h] + red[3 * HC + h]);
+                const float sum = (red_sum[h] + red_sum[HC + h]) + (red_sum[2 * HC + h] + red_sum[3 * HC + h]);
                 if (whole) {
                     const float inv = sum > 0.f ? __fdividef(1.0f, sum) : 0.f;
 #pragma unroll
@@ -817,10 +824,9 @@ __global__ void __launch_bounds__(384, 1)
                 // What the join has to do for this block: the item begun here that goes on.
                 int4 it = make_int4(-1, 0, 0, 0);
                 if (begun && !whole)  // (to the block of its last tile)
-                    it = make_int4(t.b, t.hg, paged_block(range->total, range->first + count - t.n + t.tiles - 1, range->blocks), slot);
+                    it = make_int4(t.b, t.head * a.splits + t.split, paged_block(range->total, range->first + count - t.n + t.tiles - 1, range->blocks), slot);
                 a.p.items[blockIdx.x] = it;
             }
-            ptx::named_bar_sync(bar_id, 128);  // (red is free again)
         }
         if (count == 0 && threadIdx.x == 128) a.p.items[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
