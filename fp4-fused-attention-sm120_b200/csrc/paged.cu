@@ -191,8 +191,11 @@ int encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* b
     return r == CUDA_SUCCESS ? FP4ATTN_OK : fail(FP4ATTN_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
 }
 
-// Query heads of a group computed at once (a larger group is split).
-int heads_at_once(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : group <= 16 ? 16 : 32; }
+// Query heads of a group computed at once.  A larger group is split, and its
+// keys and values are read again, from L2: 32 heads at once spilled registers
+// and took as long (144 us for 32 sequences of 1000 to 8000 tokens, 8 x 32 heads of 128;
+// 16 of them 74).
+int heads_at_once(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 
 struct AttentionWorkspace {
     size_t items, ml, o, total;
@@ -269,8 +272,7 @@ int launch_heads(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
     switch (heads_at_once(a.group)) {
         case 4: return launch_attention<OutT, D, 4>(a, blocks, join, st);
         case 8: return launch_attention<OutT, D, 8>(a, blocks, join, st);
-        case 16: return launch_attention<OutT, D, 16>(a, blocks, join, st);
-        default: return launch_attention<OutT, D, 32>(a, blocks, join, st);
+        default: return launch_attention<OutT, D, 16>(a, blocks, join, st);
     }
 }
 

@@ -65,15 +65,15 @@ namespace fp4attn {
 constexpr int kPagedBlocks = 148;
 constexpr int kPagedTile = 128;
 
-// HC: query heads computed (4, 8, 16 or 32, at least the group's share).
+// HC: query heads computed (4, 8 or 16, at least the group's share).
 template <int D, int HC, bool kSplitP>
 struct PagedCfg {
     static constexpr int THREADS = 384;
     // Tiles a step: the roles wait for one another once a step.  Tiles of
     // small heads are short, so two make a step.
     static constexpr int U = D <= 64 ? 2 : 1;
-    static constexpr int NS = HC < 16 ? 16 : HC;                     // N of the S^T MMA
-    static constexpr int NP = kSplitP ? (2 * HC < 16 ? 16 : 2 * HC) : NS;  // N of the O^T MMA: with two parts, low parts from NP / 2 on
+    static constexpr int NS = 16;                                    // N of the S^T MMA (the least there is)
+    static constexpr int NP = kSplitP && HC == 16 ? 32 : 16;         // N of the O^T MMA: with two parts, low parts from NP / 2 on
     static constexpr int KROW = D <= 64 ? 32 : D <= 128 ? 64 : 128;  // bytes of a key's codes in shared memory (= swizzle)
     static constexpr int KSTEPS = (D + 63) / 64;                     // mxf4 MMAs of K = 64 per S^T tile
     static constexpr int ATOMS = (KSTEPS + 1) / 2;                   // 512-byte scale atoms (four blocks of 32)
@@ -85,15 +85,15 @@ struct PagedCfg {
     static constexpr int DCH = D / CHE;
     static constexpr int MT = (D + 127) / 128;                       // O^T MMAs of M = 128 (rows past D are not read)
     static constexpr int PROW = 2 * NP;                              // bytes of a key's P row (= swizzle)
-    static constexpr uint32_t PSW = PROW == 32 ? ptx::kSwizzle32B : PROW == 64 ? ptx::kSwizzle64B : ptx::kSwizzle128B;
+    static constexpr uint32_t PSW = PROW == 32 ? ptx::kSwizzle32B : ptx::kSwizzle64B;
     // Tensor Memory columns
     static constexpr int S_COL = 0;                                  // [2][U][NS]
     static constexpr int O_COL = 2 * U * NS;                         // [2][MT][NP]
     static constexpr int SFA_COL = O_COL + 2 * MT * NP;
     static constexpr int SFB_COL = SFA_COL + 4 * ATOMS;
     static constexpr int TMEM_USED = SFB_COL + 4 * ATOMS;
-    static constexpr int TMEM_COLS = TMEM_USED <= 128 ? 128 : TMEM_USED <= 256 ? 256 : 512;
-    static_assert(TMEM_USED <= 512, "TMEM budget exceeded");
+    static constexpr int TMEM_COLS = TMEM_USED <= 128 ? 128 : 256;
+    static_assert(TMEM_USED <= 256, "TMEM budget exceeded");
     // shared memory, offsets from a 1024-aligned base
     static constexpr int align1k(int x) { return (x + 1023) / 1024 * 1024; }
     static constexpr int K_BYTES = kPagedTile * KROW;
@@ -611,8 +611,7 @@ __global__ void __launch_bounds__(384, 1)
         auto load_cols = [&](uint32_t col, uint32_t (&r)[HC]) {
             if constexpr (HC == 4) ptx::tmem_ld4(lanes + col, r);
             else if constexpr (HC == 8) ptx::tmem_ld8(lanes + col, r);
-            else if constexpr (HC == 16) ptx::tmem_ld16(lanes + col, r);
-            else ptx::tmem_ld32(lanes + col, r);
+            else ptx::tmem_ld16(lanes + col, r);
         };
         auto max_of = [](float x, float y) { return fmaxf(x, y); };
         auto sum_of = [](float x, float y) { return x + y; };
@@ -730,7 +729,7 @@ __global__ void __launch_bounds__(384, 1)
                             }
                         }
                         uint8_t* p = smem + C::OFF_P + (buf * C::U + u) * C::P_BYTES + row * C::PROW;
-                        const int sw = C::PROW == 32 ? (row >> 2) & 1 : C::PROW == 64 ? (row >> 1) & 3 : row & 7;
+                        const int sw = C::PROW == 32 ? (row >> 2) & 1 : (row >> 1) & 3;
                         auto put = [&](int column, const uint32_t (&v)[HC / 2]) {  // HC columns from `column` on
                             if constexpr (HC == 4) {
                                 *reinterpret_cast<uint2*>(p + (((column / 8) ^ sw) * 16)) = make_uint2(v[0], v[1]);
