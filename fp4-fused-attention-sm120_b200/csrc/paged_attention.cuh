@@ -300,15 +300,6 @@ __device__ __forceinline__ float warp_reduce4(const float (&v)[4], int lane, Op 
     return op(k, __shfl_xor_sync(~0u, k, 1));
 }
 
-// One block of 32 of a query row, quantised; out of line, for it is long and
-// runs once an item.
-static __device__ __noinline__ uint32_t quantize_query(const void* q, int64_t at, int half, int ocp, uint4* packed)
-{
-    const uint32_t sb = half ? quantize32<__half>(static_cast<const __half*>(q) + at, ocp, *packed)
-                             : quantize32<float>(static_cast<const float*>(q) + at, ocp, *packed);
-    return sb == 255u ? 254u : sb;
-}
-
 // copy(p) for pages 0 .. n - 1 of a tile, by one elected thread.  A tile's
 // whole number of pages (1, 2, 4 or 8) goes without a condition on each copy:
 // with one, a copy took 85 cycles to issue instead of 20.
@@ -630,13 +621,25 @@ __global__ void __launch_bounds__(384, 1)
             // (S^T of this warpgroup's last item, the buffer's last use, is computed.)
             {
                 const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(t.head) * a.group + h0) * a.qh;
-                for (int k = row; k < nh * C::NB; k += 128) {
-                    const int r = k / C::NB, blk = k % C::NB;
-                    uint4 packed;
-                    const uint32_t sb = quantize_query(a.q, q0 + r * a.qh + blk * 32, a.q_half, a.ocp, &packed);
+                for (int k = row; k < nh * C::NB * 4; k += 128) {  // a thread per eight elements
+                    const int r = k / (C::NB * 4), blk = k / 4 % C::NB, quarter = k % 4;
+                    const int64_t at = q0 + r * a.qh + blk * 32 + quarter * 8;
+                    float v[8];
+                    if (a.q_half) load8v(static_cast<const __half*>(a.q) + at, v);
+                    else load8v(static_cast<const float*>(a.q) + at, v);
+                    float amax = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(v[e]));
+                    const uint32_t quad = 0xFu << (lane & ~3);
+                    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+                    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+                    const uint32_t sb = scale_byte(amax, a.ocp);
+                    // (exact for FP16 too; the quantiser's FP16 path is only faster)
+                    const uint32_t codes = encode8<float>(v, sb);
                     const int sw = C::KROW == 32 ? (r >> 2) & 1 : C::KROW == 64 ? (r >> 1) & 3 : r & 7;
-                    *reinterpret_cast<uint4*>(smem + C::OFF_Q + wg * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16)) = packed;
-                    smem[C::OFF_QSF + (wg * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb);
+                    *reinterpret_cast<uint32_t*>(smem + C::OFF_Q + wg * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16) + quarter * 4) = codes;
+                    if (quarter == 0)
+                        smem[C::OFF_QSF + (wg * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb == 255u ? 254u : sb);
                 }
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(&q_full[wg]);
