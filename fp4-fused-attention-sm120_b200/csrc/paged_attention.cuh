@@ -300,28 +300,61 @@ __device__ __forceinline__ float warp_reduce4(const float (&v)[4], int lane, Op 
     return op(k, __shfl_xor_sync(~0u, k, 1));
 }
 
-// copy(p) for pages 0 .. n - 1 of a tile, by one elected thread.  A tile's
-// whole number of pages (1, 2, 4 or 8) goes without a condition on each copy:
-// with one, a copy took 85 cycles to issue instead of 20.
+// What runs once an item or less is out of line: the roles' loops together just
+// about fill the SM's instruction cache, and with the rest between them they
+// took up to a quarter longer.
+
+// Eight elements of a query row, quantised with those of the three neighbouring
+// lanes: their codes, and the block's scale byte.  (encode8<float> is exact for
+// FP16 too.)
+static __device__ __noinline__ uint2 quantize_query8(const void* q, int64_t at, int half, int ocp)
+{
+    float v[8];
+    if (half) load8v(static_cast<const __half*>(q) + at, v);
+    else load8v(static_cast<const float*>(q) + at, v);
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(v[e]));
+    const uint32_t quad = 0xFu << ((threadIdx.x & 31) & ~3);
+    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+    const uint32_t sb = scale_byte(amax, ocp);
+    return make_uint2(encode8<float>(v, sb), sb == 255u ? 254u : sb);
+}
+
+// Zeroes V of keys [keys, end) of a stage's tile: thread `row` of 128.
+template <int D, int CB>
+__device__ __noinline__ void zero_keys(uint8_t* v, int keys, int end, int page, int shift, int row)
+{
+    for (int k = row; k < (end - keys) * (D / 8); k += 128) {
+        const int key = keys + k / (D / 8), c = k % (D / 8);
+        *reinterpret_cast<uint4*>(v + (key >> shift) * page * D * 2 + c / (CB / 16) * page * CB + (key & (page - 1)) * CB +
+                                  c % (CB / 16) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
+// copy(p, id[p]) for pages 0 .. n - 1 of a tile (at most 8), by one elected
+// thread, in runs of 8, 4, 2 and 1.  With a condition on each copy, one took 85
+// cycles to issue instead of 20.
 template <typename F>
-__device__ __forceinline__ void each_page(int n, F copy)
+__device__ __forceinline__ void each_page(int n, const int (&id)[8], F copy)
 {
     if (n == 8) {
 #pragma unroll
-        for (int p = 0; p < 8; p++) copy(p);
-    } else if (n == 4) {
-#pragma unroll
-        for (int p = 0; p < 4; p++) copy(p);
-    } else if (n == 2) {
-        copy(0);
-        copy(1);
-    } else if (n == 1) {
-        copy(0);
-    } else {
-#pragma unroll
-        for (int p = 0; p < 7; p++)
-            if (p < n) copy(p);
+        for (int p = 0; p < 8; p++) copy(p, id[p]);
+        return;
     }
+    const bool four = n & 4;
+    if (four) {
+#pragma unroll
+        for (int p = 0; p < 4; p++) copy(p, id[p]);
+    }
+    if (n & 2) {
+        copy(four ? 4 : 0, four ? id[4] : id[0]);
+        copy(four ? 5 : 1, four ? id[5] : id[1]);
+    }
+    const int last = n & 6;
+    if (n & 1) copy(last, last == 0 ? id[0] : last == 2 ? id[2] : last == 4 ? id[4] : id[6]);
 }
 
 template <typename OutT, int D, int HC>
@@ -432,15 +465,15 @@ __global__ void __launch_bounds__(384, 1)
                 if (ptx::elect_one()) {
                     if (keys_role) {
                         ptx::mbar_arrive_expect_tx(&k_full[ring.s], n * page * (C::KROW + C::NB));
-                        each_page(n, [&](int p) {
-                            ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, pid[p]);
-                            ptx::bulk_load(st + C::K_BYTES + C::V_BYTES + p * page * C::NB, scales + pid[p] * a.c.k_scales_stride,
+                        each_page(n, pid, [&](int p, int at) {
+                            ptx::tma_load_4d(st + p * page * C::KROW, &tm_k, &k_full[ring.s], 0, head, at);
+                            ptx::bulk_load(st + C::K_BYTES + C::V_BYTES + p * page * C::NB, scales + at * a.c.k_scales_stride,
                                            page * C::NB, &k_full[ring.s]);
                         });
                     } else {
                         ptx::mbar_arrive_expect_tx(&v_full[ring.s], n * page * D * 2);
-                        each_page(n, [&](int p) {
-                            ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, pid[p]);
+                        each_page(n, pid, [&](int p, int at) {
+                            ptx::tma_load_5d(st + C::K_BYTES + p * page * D * 2, &tm_v, &v_full[ring.s], 0, 0, head, at);
                         });
                     }
                 }
@@ -623,23 +656,10 @@ __global__ void __launch_bounds__(384, 1)
                 const int64_t q0 = t.b * a.qb + (static_cast<int64_t>(t.head) * a.group + h0) * a.qh;
                 for (int k = row; k < nh * C::NB * 4; k += 128) {  // a thread per eight elements
                     const int r = k / (C::NB * 4), blk = k / 4 % C::NB, quarter = k % 4;
-                    const int64_t at = q0 + r * a.qh + blk * 32 + quarter * 8;
-                    float v[8];
-                    if (a.q_half) load8v(static_cast<const __half*>(a.q) + at, v);
-                    else load8v(static_cast<const float*>(a.q) + at, v);
-                    float amax = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(v[e]));
-                    const uint32_t quad = 0xFu << (lane & ~3);
-                    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
-                    amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
-                    const uint32_t sb = scale_byte(amax, a.ocp);
-                    // (exact for FP16 too; the quantiser's FP16 path is only faster)
-                    const uint32_t codes = encode8<float>(v, sb);
+                    const uint2 q8 = quantize_query8(a.q, q0 + r * a.qh + blk * 32 + quarter * 8, a.q_half, a.ocp);
                     const int sw = C::KROW == 32 ? (r >> 2) & 1 : C::KROW == 64 ? (r >> 1) & 3 : r & 7;
-                    *reinterpret_cast<uint32_t*>(smem + C::OFF_Q + wg * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16) + quarter * 4) = codes;
-                    if (quarter == 0)
-                        smem[C::OFF_QSF + (wg * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(sb == 255u ? 254u : sb);
+                    *reinterpret_cast<uint32_t*>(smem + C::OFF_Q + wg * C::Q_BYTES + r * C::KROW + ((blk ^ sw) * 16) + quarter * 4) = q8.x;
+                    if (quarter == 0) smem[C::OFF_QSF + (wg * C::ATOMS + blk / 4) * 512 + r * 16 + blk % 4] = static_cast<uint8_t>(q8.y);
                 }
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(&q_full[wg]);
@@ -746,16 +766,12 @@ __global__ void __launch_bounds__(384, 1)
                         put(0, hi);
                         if constexpr (kSplitP) put(C::NP / 2, lo);
                         const int keys = t.keys(i * C::U + u);
-                        if (keys < kPagedTile) {
-                            if (row >= keys && row < max(16, (keys + 15) / 16 * 16)) {
-                                // A key behind the last: whatever lies in its place of V
-                                // (NaN included) must not meet its weight of zero.
-                                ok = bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull) && ok;
-                                uint8_t* v = stages + ring.s * C::STAGE + C::K_BYTES + (row >> shift) * page * D * 2 + (row & (page - 1)) * C::CB;
-#pragma unroll 1
-                                for (int c = 0; c < C::DCH * (C::CB / 16); c++)
-                                    *reinterpret_cast<uint4*>(v + c / (C::CB / 16) * page * C::CB + c % (C::CB / 16) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                            }
+                        if (keys % 16 != 0 || keys == 0) {
+                            // Keys behind the last, up to the end of its MMA step:
+                            // whatever lies in their places of V (NaN included) must
+                            // not meet their weights of zero.
+                            ok = bounded_wait(&v_full[ring.s], ring.parity, w, kPagedVFull) && ok;
+                            zero_keys<D, C::CB>(stages + ring.s * C::STAGE + C::K_BYTES, keys, max(16, (keys + 15) / 16 * 16), page, shift, row);
                         }
                         ring.next();
                     }
