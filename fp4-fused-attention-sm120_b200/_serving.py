@@ -1,13 +1,10 @@
 """What rotary.py and paged.py share: the library's handle with their
-prototypes, argument checks, and the device and stream of a launch."""
+prototypes, the binding of their tensor calls, and the stream of a launch."""
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import fp4attn_b200 as _fa
-
-F32, F16 = 0, 1
 
 
 class CacheStruct(ctypes.Structure):
@@ -37,9 +34,7 @@ def declare(L) -> None:
 
 
 lib, check, scale_mode = _fa.lib, _fa._check, _fa._scale_mode
-I2, I3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
-_T = None
-_CODES = {}
+_T = _NATIVE = None
 
 
 def torch():
@@ -48,49 +43,28 @@ def torch():
     global _T
     if _T is None:
         _T = _fa._torch()
-        _CODES.update({_T.float16: F16, _T.float32: F32})
     return _T
 
 
-def dtype_code(dtype) -> int:
-    torch()
-    code = _CODES.get(dtype)
-    if code is None:
-        raise TypeError(f"unsupported dtype {dtype}; use float16 or float32")
-    return code
-
-
-def check_index(t, name, device):
-    if t.dtype is not torch().int32 or t.device != device:
-        raise ValueError(f"{name} must be an int32 tensor on {device}")
-
-
-def check_table(table, device, head_dim):
-    """(pointer, rotary_dim, positions) of a rotary table."""
-    shape = table.shape
-    if (len(shape) != 3 or shape[2] != 2 or table.dtype is not torch().float32 or table.device != device or
-            not table.is_contiguous()):
-        raise ValueError(f"table must be a contiguous float32 [positions, rotary_dim / 2, 2] tensor on {device}")
-    if 2 * shape[1] > head_dim:
-        raise ValueError(f"the table's rotary_dim {2 * shape[1]} exceeds head_dim {head_dim}")
-    return table.data_ptr(), 2 * shape[1], shape[0]
-
-
-_HERE = contextlib.nullcontext()
+def native():
+    """The binding of the tensor calls (csrc/binding.cpp), bound to the library."""
+    global _NATIVE
+    if _NATIVE is None:
+        torch()
+        L = lib()
+        try:
+            from . import _native
+        except ImportError as e:
+            raise ImportError(f"{e}: build it with `make -C csrc` in the package directory "
+                              "(there is no fallback implementation)") from e
+        names = ("rotary", "cache_append", "cache_gather", "paged_attention_workspace_size", "paged_attention", "copy_pages")
+        _native.bind(check, *[ctypes.cast(getattr(L, "fp4attn_" + n), ctypes.c_void_p).value for n in names])
+        _NATIVE = _native
+    return _NATIVE
 
 
 def on(device, stream):
-    """Context in which a call allocates and launches: the tensors' device
-    current, and `stream` (default: that device's current stream) the stream
-    its outputs and workspaces belong to."""
-    T = torch()
-    if stream is not None:
-        if stream.device != device:
-            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-        return T.cuda.stream(stream)
-    return _HERE if device.index == T.cuda.current_device() else T.cuda.device(device)
-
-
-def stream_ptr(device) -> int:
-    """The current stream of a device, as the library takes it."""
-    return _T._C._cuda_getCurrentRawStream(device.index)
+    """Context of a call on `stream`, which its outputs and workspaces belong to."""
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+    return torch().cuda.stream(stream)

@@ -56,6 +56,7 @@ class PagedCache:
                                      max(k_codes.stride(0), k_codes[0].numel()),
                                      max(k_scales.stride(0), k_scales[0].numel()),
                                      2 * max(v.stride(0), v[0].numel()), P, S, H, D)
+        self._at = ctypes.addressof(self.struct)
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, device="cuda"):
@@ -67,33 +68,6 @@ class PagedCache:
                    torch.empty(shape + (head_dim,), dtype=torch.float16, device=device))
 
 
-def _check_block_table(block_table, device):
-    """(pointer, row stride, sequences, pages) of a block table."""
-    sv.check_index(block_table, "block_table", device)
-    shape, strides = block_table.shape, block_table.stride()
-    if len(shape) != 2 or shape[1] < 1 or strides[1] != 1:
-        raise ValueError("block_table must be [sequences, pages] with contiguous rows")
-    n, pages = shape
-    return block_table.data_ptr(), strides[0] if n > 1 else pages, n, pages
-
-
-def _check_vector(t, name, n, device):
-    sv.check_index(t, name, device)
-    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be a contiguous int32 [{n}] tensor")
-    return t.data_ptr()
-
-
-def _check_rows(t, name, tokens, heads, cache, dtype):
-    """(token, head) strides of a [tokens, heads, head_dim] tensor; heads=None: any number."""
-    shape, strides = t.shape, t.stride()
-    if (len(shape) != 3 or shape[0] != tokens or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads) or
-            t.device != cache.device or t.dtype is not dtype or strides[2] != 1):
-        raise ValueError(f"{name} must be a [{tokens}, {heads or 'heads'}, {cache.head_dim}] {dtype} tensor on "
-                         f"{cache.device} with a contiguous last dimension")
-    return sv.I2(strides[0], strides[1])
-
-
 def cache_append(cache, K, V, block_table, positions, seq_ids=None, Q=None, table=None, interleaved=False,
                  scale_mode="reference", stream=None):
     """Puts tokens into the cache (fp4attn_cache_append): K and V [tokens,
@@ -103,25 +77,12 @@ def cache_append(cache, K, V, block_table, positions, seq_ids=None, Q=None, tabl
     rotated by their positions first.  With Q [tokens, heads, head_dim] returns
     the queries rotated the same way, contiguous.  No two tokens of a call may
     have the same place in the cache."""
-    torch = sv.torch()
-    tokens, dtype, device = K.shape[0], K.dtype, cache.device
-    code, rule = sv.dtype_code(dtype), sv.scale_mode(scale_mode)
-    ks = _check_rows(K, "K", tokens, cache.kv_heads, cache, dtype)
-    vs = _check_rows(V, "V", tokens, cache.kv_heads, cache, dtype)
-    qs = None if Q is None else _check_rows(Q, "Q", tokens, None, cache, dtype)
-    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, device)
-    pos = _check_vector(positions, "positions", tokens, device)
-    ids = None if seq_ids is None else _check_vector(seq_ids, "seq_ids", tokens, device)
-    tab = (None, 0, 0) if table is None else sv.check_table(table, device, cache.head_dim)
-    with sv.on(device, stream):
-        out, q_ptr, out_ptr, q_heads = None, None, None, 0
-        if Q is not None:
-            out, q_ptr, q_heads = torch.empty(Q.shape, dtype=dtype, device=device), Q.data_ptr(), Q.shape[1]
-            out_ptr = out.data_ptr()
-        sv.check(sv.lib().fp4attn_cache_append(
-            cache.struct, K.data_ptr(), V.data_ptr(), q_ptr, out_ptr, code, tokens, q_heads, ks, vs, qs, bt, bt_stride,
-            seqs, max_pages, ids, pos, *tab, interleaved, rule, sv.stream_ptr(device)), "fp4attn_cache_append")
-    return out
+    args = (cache._at, cache.device.index, K, V, block_table, positions, seq_ids, Q, table, interleaved,
+            sv.scale_mode(scale_mode))
+    if stream is None:
+        return sv.native().cache_append(*args)
+    with sv.on(cache.device, stream):
+        return sv.native().cache_append(*args)
 
 
 def cache_gather(cache, block_table, starts, lengths, max_length, heads=None, dtype=None, stream=None):
@@ -130,21 +91,11 @@ def cache_gather(cache, block_table, starts, lengths, max_length, heads=None, dt
     behind them (fp4attn_cache_gather).  starts=None reads from token 0; heads
     (default: the cache's) repeats each key/value head for its query heads, as
     fused_fp4_attention wants them."""
-    torch = sv.torch()
-    device = cache.device
-    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, device)
-    st = None if starts is None else _check_vector(starts, "starts", seqs, device)
-    ln = _check_vector(lengths, "lengths", seqs, device)
-    heads = cache.kv_heads if heads is None else heads
-    dtype = dtype or torch.float16
-    code = sv.dtype_code(dtype)
-    with sv.on(device, stream):
-        K = torch.empty((seqs, heads, max_length, cache.head_dim), dtype=dtype, device=device)
-        V = torch.empty_like(K)
-        sv.check(sv.lib().fp4attn_cache_gather(cache.struct, bt, bt_stride, seqs, max_pages, st, ln, max_length, heads,
-                                               K.data_ptr(), V.data_ptr(), code, sv.stream_ptr(device)),
-                 "fp4attn_cache_gather")
-    return K, V
+    args = (cache._at, cache.device.index, block_table, starts, lengths, max_length, heads, dtype)
+    if stream is None:
+        return sv.native().cache_gather(*args)
+    with sv.on(cache.device, stream):
+        return sv.native().cache_gather(*args)
 
 
 def paged_attention_workspace_size(cache, batch, heads):
@@ -154,37 +105,12 @@ def paged_attention_workspace_size(cache, batch, heads):
 
 
 def _attend(Q, cache, block_table, seq_lens, softmax_scale, scale_mode, out_dtype, out, with_lse, workspace, stream):
-    torch = sv.torch()
-    dtype, device = Q.dtype, cache.device
-    code, rule = sv.dtype_code(dtype), sv.scale_mode(scale_mode)
-    qs = _check_rows(Q, "Q", Q.shape[0], None, cache, dtype)
-    B, H, D = Q.shape
-    bt, bt_stride, seqs, max_pages = _check_block_table(block_table, device)
-    if seqs != B:
-        raise ValueError(f"block_table has {seqs} rows for {B} queries")
-    ln = _check_vector(seq_lens, "seq_lens", B, device)
-    if out is None:
-        out_code = code if out_dtype is None else sv.dtype_code(out_dtype)
-    else:
-        out_code = sv.dtype_code(out.dtype)
-        if (out.shape != Q.shape or not out.is_contiguous() or out.device != device or
-                (out_dtype is not None and out.dtype != out_dtype)):
-            raise ValueError("out must be contiguous with Q's shape, on its device")
-    if workspace is not None and (workspace.device != device or workspace.dtype is not torch.uint8 or
-                                  not workspace.is_contiguous()):
-        raise ValueError("workspace must be a contiguous uint8 tensor on Q's device")
-    with sv.on(device, stream):
-        if out is None:
-            out = torch.empty((B, H, D), dtype=out_dtype or dtype, device=device)
-        lse = torch.empty((B, H), dtype=torch.float32, device=device) if with_lse else None
-        if workspace is None:
-            workspace = torch.empty(max(1, paged_attention_workspace_size(cache, B, H)), dtype=torch.uint8,
-                                    device=device)
-        sv.check(sv.lib().fp4attn_paged_attention(
-            cache.struct, Q.data_ptr(), out.data_ptr(), lse.data_ptr() if with_lse else None, code, out_code, B, H, qs,
-            bt, bt_stride, max_pages, ln, softmax_scale or 0.0, rule, workspace.data_ptr(), workspace.numel(),
-            sv.stream_ptr(device)), "fp4attn_paged_attention")
-    return out, lse
+    args = (Q, cache._at, cache.device.index, block_table, seq_lens, softmax_scale, sv.scale_mode(scale_mode),
+            out_dtype, out, with_lse, workspace)
+    if stream is None:
+        return sv.native().attend(*args)
+    with sv.on(cache.device, stream):
+        return sv.native().attend(*args)
 
 
 def paged_attention(Q, cache, block_table, seq_lens, softmax_scale=None, scale_mode="reference", out_dtype=None,
@@ -198,7 +124,7 @@ def paged_attention(Q, cache, block_table, seq_lens, softmax_scale=None, scale_m
     paged_attention_workspace_size bytes, not shared by calls in flight at once)
     to allocate nothing."""
     return _attend(Q, cache, block_table, seq_lens, softmax_scale, scale_mode, out_dtype, out, False, workspace,
-                   stream)[0]
+                   stream)
 
 
 def paged_attention_lse(Q, cache, block_table, seq_lens, softmax_scale=None, scale_mode="reference", out_dtype=None,
@@ -219,17 +145,13 @@ def copy_pages(caches, src, dst, stream=None):
     if not caches:
         return
     device = caches[0].device
-    src, dst = _page_numbers(src, "src"), _page_numbers(dst, "dst")
-    n = src.shape[0]
-    if n != dst.shape[0]:
-        raise ValueError("src and dst differ in length")
-    structs = (sv.CacheStruct * len(caches))(*[c.struct for c in caches])
-    for c in caches:
-        if c.device != device:
-            raise ValueError("the caches must be on one device")
+    if any(c.device != device for c in caches):
+        raise ValueError("the caches must be on one device")
+    args = ([c._at for c in caches], device.index, _page_numbers(src, "src"), _page_numbers(dst, "dst"))
+    if stream is None:
+        return sv.native().copy_pages(*args)
     with sv.on(device, stream):
-        sv.check(sv.lib().fp4attn_copy_pages(structs, len(caches), src.data_ptr(), dst.data_ptr(), n,
-                                             sv.stream_ptr(device)), "fp4attn_copy_pages")
+        sv.native().copy_pages(*args)
 
 
 def _page_numbers(pages, name):
@@ -237,15 +159,11 @@ def _page_numbers(pages, name):
     torch = sv.torch()
     if not isinstance(pages, torch.Tensor):
         pages = torch.tensor(pages, dtype=torch.int64)
-    if pages.dtype is not torch.int32:
-        if pages.dtype is not torch.int64:
-            raise ValueError(f"{name} must be int32 or int64")
+    if pages.dtype is torch.int64 and not pages.is_cuda:
         narrow = pages.to(torch.int32)
         if not torch.equal(narrow.to(torch.int64), pages):
             raise ValueError(f"{name}: page number out of range")
         pages = narrow
-    if pages.dim() != 1 or pages.is_cuda:
-        raise ValueError(f"{name} must be page numbers in host memory")
     return pages.contiguous()
 
 

@@ -76,10 +76,10 @@ def rotary_table(max_positions, rotary_dim, base=10000.0, scaling=None, factor=1
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     arr = (ctypes.c_double * len(freqs))(*freqs)
-    with sv.on(device, stream):
+    with torch.cuda.device(device) if stream is None else sv.on(device, stream):
         table = torch.empty((max_positions, rotary_dim // 2, 2), dtype=torch.float32, device=device)
         sv.check(sv.lib().fp4attn_rotary_table(arr, len(freqs), max_positions, table_factor, table.data_ptr(),
-                                               sv.stream_ptr(device)), "fp4attn_rotary_table")
+                                               torch.cuda.current_stream().cuda_stream), "fp4attn_rotary_table")
     return table
 
 
@@ -91,33 +91,11 @@ def rotary(x, table, positions=None, interleaved=False, inverse=False, out=None,
     positions: int32 [seq] or [batch, seq], by default 0 .. seq - 1.
     interleaved: pairs (2j, 2j + 1) instead of (j, j + rotary_dim / 2).
     inverse: turn back, which is the gradient's rotation."""
-    torch = sv.torch()
-    device, dtype, strides = x.device, x.dtype, x.stride()
-    if len(strides) != 4 or not x.is_cuda or strides[3] != 1:
-        raise ValueError("x must be a [batch, heads, seq, head_dim] CUDA tensor with a contiguous last dimension")
-    B, H, S, D = x.shape
-    code = sv.dtype_code(dtype)
-    table_ptr, rotary_dim, max_positions = sv.check_table(table, device, D)
-    pos_ptr, pos_stride = None, 0
-    if positions is not None:
-        sv.check_index(positions, "positions", device)
-        if positions.dim() == 2 and positions.shape == (B, S):
-            pos_stride = positions.stride(0)
-        elif positions.shape != (S,):
-            raise ValueError("positions must be [seq] or [batch, seq]")
-        if S > 1 and positions.stride(-1) != 1:
-            raise ValueError("positions must be contiguous along seq")
-        pos_ptr = positions.data_ptr()
-    if out is not None and (out.shape != x.shape or out.dtype != dtype or out.device != device or out.stride(3) != 1):
-        raise ValueError("out must have x's shape, dtype and device, and a contiguous last dimension")
-    with sv.on(device, stream):
-        if out is None:
-            out = torch.empty((B, H, S, D), dtype=dtype, device=device)
-        sv.check(sv.lib().fp4attn_rotary(
-            x.data_ptr(), out.data_ptr(), code, B, H, S, D, sv.I3(*strides[:3]), sv.I3(*out.stride()[:3]), table_ptr,
-            rotary_dim, max_positions, pos_ptr, pos_stride, interleaved, inverse, sv.stream_ptr(device)),
-            "fp4attn_rotary")
-    return out
+    native = sv.native()
+    if stream is None:
+        return native.rotary(x, table, positions, interleaved, inverse, out)
+    with sv.on(x.device, stream):
+        return native.rotary(x, table, positions, interleaved, inverse, out)
 
 
 _ROTARY_FN = None
