@@ -443,7 +443,8 @@ int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table,
     if (bad_dtype(dtype)) return fail(FP4ATTN_EINVAL, "dtype %d", dtype);
     if (int rc = check_table(block_table, table_stride, seqs, max_pages)) return rc;
     if (heads < 1 || heads % cache->kv_heads) return fail(FP4ATTN_EINVAL, "heads %d is not a multiple of kv_heads %d", heads, cache->kv_heads);
-    if (max_length < 0 || seqs > 65535) return fail(FP4ATTN_EINVAL, "max_length >= 0, at most 65535 sequences");
+    if (max_length < 0 || max_length > (1 << 30) || seqs > 65535)
+        return fail(FP4ATTN_EINVAL, "max_length in [0, 2^30], at most 65535 sequences");
     if (seqs == 0 || max_length == 0) return FP4ATTN_OK;
     if (!lengths || !K || !V || !aligned(K, 16) || !aligned(V, 16) || !aligned(lengths, 4) || !aligned(starts, 4) ||
         !aligned(block_table, 4))
@@ -480,6 +481,12 @@ int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out
     if (q_heads < 1 || q_heads % cache->kv_heads)
         return fail(FP4ATTN_EINVAL, "q_heads %d is not a multiple of kv_heads %d", q_heads, cache->kv_heads);
     if (int rc = check_table(block_table, table_stride, batch, max_pages)) return rc;
+    // (the device counts tokens and tiles in 32 bits)
+    if (static_cast<int64_t>(max_pages) * cache->page_size > (1 << 30))
+        return fail(FP4ATTN_EINVAL, "max_pages %d of %d tokens: more than 2^30", max_pages, cache->page_size);
+    const int64_t longest = (static_cast<int64_t>(max_pages) * cache->page_size + kPagedTile - 1) / kPagedTile;
+    const int64_t most_tiles = longest * q_heads * batch;
+    if (most_tiles > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "batch %d x heads %d x max_pages %d: more than 2^31 tiles", batch, q_heads, max_pages);
     if (batch == 0) return FP4ATTN_OK;
     if (!Q || !Out || !q_strides || !seq_lens) return fail(FP4ATTN_EINVAL, "null pointer");
     if (!wide(Q, in_dtype, {q_strides[0], q_strides[1]}) || !aligned(Out, 16) || !aligned(lse, 4) || !aligned(seq_lens, 4) ||
@@ -516,9 +523,6 @@ int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out
                         reinterpret_cast<int4*>(base + ws.items)};
     a.timeout_ns = host::timeout_ns();
     // The most tiles the block table allows; what there are is known on the device.
-    const int64_t longest = (static_cast<int64_t>(max_pages) * cache->page_size + kPagedTile - 1) / kPagedTile;
-    if (longest * a.head_groups > 0x7FFFFFFF / batch)
-        return fail(FP4ATTN_EINVAL, "batch %d x heads x max_pages %d has more than 2^31 tiles", batch, max_pages);
     const int64_t tiles = longest * a.head_groups * batch;
     const int blocks = static_cast<int>(std::min<int64_t>({kPagedBlocks, host::sms(), tiles}));
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -127,5 +127,9 @@ def _autograd_function():
 
 
 def rotary_embedding(x, table, positions=None, interleaved=False):
-    """``rotary`` that autograd can differentiate (with respect to x)."""
+    """``rotary`` that autograd can differentiate (with respect to x).
+
+    As with every operation: when a backward pass is captured into a CUDA
+    graph, no eager graph of the same leaves may be alive, for autograd would
+    wait for the stream of that one, which ends the capture."""
     return _autograd_function().apply(x, table, positions, interleaved)

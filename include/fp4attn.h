@@ -337,7 +337,10 @@ typedef struct {
  * query row; so does a position beyond the rotary table, as FP4ATTN_EINDEX.
  * The codes and scales are byte for byte those of fp4attn_rotary followed by
  * fp4attn_quantize.  No two tokens of a call may have the same place in the
- * cache. */
+ * cache, and Q_out must not overlap Q.  One block a token in parallel: rows are
+ * fastest 16-byte aligned (pointers and strides) with rotary_dim a multiple of
+ * 64, or interleaved and a multiple of 8; every other form is taken element by
+ * element. */
 int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* V, const void* Q, void* Q_out,
                          int dtype, int tokens, int q_heads, const int64_t* k_strides, const int64_t* v_strides,
                          const int64_t* q_strides, const int32_t* block_table, int64_t table_stride, int seqs,
@@ -366,7 +369,13 @@ size_t fp4attn_paged_attention_workspace_size(int batch, int q_heads, int kv_hea
  * lse (or null): [batch, q_heads] natural log-sum-exp.  A sequence of length
  * 0 gives zeros and +inf.  Several new tokens of one sequence are as many
  * rows that share its pages, with lengths that grow by one.
- * softmax_scale <= 0 selects 1/sqrt(head_dim).  workspace: as
+ * softmax_scale <= 0 selects 1/sqrt(head_dim).  FP16 output: the probabilities
+ * are rounded to FP16 once, as in the forward; FP32 output: they keep 22 bits.
+ * A length beyond the block table counts as the table's, and a page outside the
+ * cache as page 0 (FP4ATTN_EINDEX either way; the other sequences keep their
+ * results).  max_pages * page_size is at most 2^30.  Results repeat bit for bit
+ * for the same lengths; they depend on the lengths of the other sequences in the
+ * last bits, by where long sequences are divided.  workspace: as
  * fp4attn_paged_attention_workspace_size says, 256-byte aligned, any content;
  * not shared with another call in flight. */
 int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out, float* lse, int in_dtype,

@@ -89,6 +89,7 @@ def test_attention_refuses_bad_arguments(fa):
     assert _attend(fa, qh=3) == fa.EINVAL                       # not a multiple of the cache's two
     assert _attend(fa, batch=-1) == fa.EINVAL
     assert _attend(fa, maxp=0) == fa.EINVAL
+    assert _attend(fa, maxp=1 << 25, bts=1 << 25) == fa.EINVAL  # 2^31 tokens
     assert _attend(fa, lens=None) == fa.EINVAL
     assert _attend(fa, Q=24) == fa.EINVAL
     assert _attend(fa, qs=I2(512, 132)) == fa.EINVAL
@@ -108,6 +109,7 @@ def test_gather_refuses_bad_arguments(fa):
     assert _gather(fa, dt=2) == fa.EINVAL
     assert _gather(fa, heads=3) == fa.EINVAL
     assert _gather(fa, most=-1) == fa.EINVAL
+    assert _gather(fa, most=(1 << 30) + 1) == fa.EINVAL
     assert _gather(fa, lens=None) == fa.EINVAL
     assert _gather(fa, K=8) == fa.EINVAL
     assert _gather(fa, seqs=0) == fa.OK

@@ -124,6 +124,29 @@ def test_rotary_positions_out_of_range(fa, cuda):
     assert torch.equal(y[:, :, :1], fa.rotary(x[:, :, :1], table, torch.tensor([7], dtype=torch.int32).cuda()))
 
 
+def test_rotary_gradient_under_capture(fa, cuda):
+    """Forward and gradient captured (no eager graph of the leaf alive) and replayed on new inputs."""
+    table = fa.rotary_table(64, 64)
+    x = torch.randn(1, 2, 64, 64, generator=_gen(1)).cuda().requires_grad_()
+    dy = torch.randn(1, 2, 64, 64, generator=_gen(2)).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # (autograd's own warm-up)
+        torch.autograd.grad(fa.rotary_embedding(x, table), x, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = fa.rotary_embedding(x, table)
+        (dx,) = torch.autograd.grad(y, x, dy)
+        y = y.detach()
+    with torch.no_grad():
+        x.copy_(torch.randn(1, 2, 64, 64, generator=_gen(3)))
+        dy.copy_(torch.randn(1, 2, 64, 64, generator=_gen(4)))
+    g.replay()
+    assert torch.equal(y, fa.rotary(x.detach(), table))
+    assert torch.equal(dx, fa.rotary(dy, table, inverse=True))
+
+
 def test_rotary_under_capture(fa, cuda):
     table = fa.rotary_table(64, 64)
     x = torch.randn(1, 2, 64, 64, generator=_gen(1)).half().cuda()
@@ -164,6 +187,23 @@ APPEND = [  # page, kv_heads, q_heads, D, rotary_dim, dtype, interleaved, ocp
     (16, 1, 2, 256, 256, F32, True, False),
     (64, 4, 4, 32, 0, F16, False, False),
 ]
+
+
+def test_append_of_unaligned_rows(fa, cuda):
+    """Rows off a 16-byte boundary and odd strides: the bytes of aligned rows."""
+    for r, inter in ((64, False), (64, True), (0, False), (24, True)):
+        base = torch.randn(9, 3, 64 + 5, generator=_gen(4)).half().cuda()
+        x = base[:, :, 3:67]
+        table = fa.rotary_table(32, r) if r else None
+        got = []
+        for t in (x, x.contiguous()):
+            c = _blank(fa, 2, 16, 3, 64)
+            q = fa.cache_append(c, t, t, torch.tensor([[1, 0]]).int().cuda(), torch.arange(9).int().cuda() + 11,
+                                torch.zeros(9).int().cuda(), Q=t, table=table, interleaved=inter)
+            got.append((q, *_cpu(c)))
+        for a, b in zip(*got):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert fa.status_query() == fa.OK
 
 
 @pytest.mark.parametrize("case", APPEND)
@@ -521,6 +561,50 @@ def test_attention_captured_with_growing_lengths(fa, cuda):
         graph.replay()
         assert torch.equal(out, fa.paged_attention(fa.rotary(q.transpose(0, 1)[None], table, pos)[0].transpose(0, 1).contiguous(),
                                                    c, bt, lens))
+    assert fa.status_query() == fa.OK
+
+
+def test_two_captured_calls_share_a_workspace(fa, cuda):
+    """Graphs of different calls over one workspace, replayed in turn: each gives its own result every time."""
+    c = _filled(fa, 5, 400, 64, 2, 128)
+    bt = _tables(1, 4, 100, 400).cuda()
+    ws = torch.empty(fa.paged_attention_workspace_size(c, 4, 8), dtype=torch.uint8, device="cuda")
+    calls = []
+    for seed, lens in ((1, [6000, 3, 0, 1234]), (2, [1, 6400, 6400, 77])):
+        q, ln = torch.randn(4, 8, 128, generator=_gen(seed)).half().cuda(), torch.tensor(lens).int().cuda()
+        want = fa.paged_attention(q, c, bt, ln)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fa.paged_attention(q, c, bt, ln, workspace=ws)
+        calls.append((graph, out, want, q, ln))  # (the graph reads q and ln where they are)
+    for _ in range(3):
+        for graph, out, want, *_ in calls:
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+    assert fa.status_query() == fa.OK
+
+
+def test_caches_past_32_bit_offsets(fa, cuda):
+    """Pages whose values, codes and scales lie 4 GiB and more into their tensors."""
+    P, hk, page, D = 70000, 8, 64, 128              # 9.2 GB of values, 2.3 GB of codes
+    c = fa.PagedCache.empty(P, page, hk, D)
+    bt = torch.tensor([[P - 1, 5, P - 3], [P - 2, 40000, 33000]], dtype=torch.int32)
+    n = 3 * page - 7
+    kv = torch.randn(2 * n, 2 * hk, D, generator=_gen(1)).half()
+    pos, ids = torch.arange(n).int().repeat(2), torch.repeat_interleave(torch.arange(2), n).int()
+    d = kv.cuda()
+    fa.cache_append(c, d[:, :hk], d[:, hk:], bt.cuda(), pos.cuda(), ids.cuda())
+    lens = torch.full((2,), n).int().cuda()
+    K, V = fa.cache_gather(c, bt.cuda(), None, lens, n)
+    assert torch.equal(V, d[:, hk:].view(2, n, hk, D).transpose(1, 2))
+    q = torch.randn(2, hk, D, generator=_gen(2)).half()
+    out = fa.paged_attention(q.cuda(), c, bt.cuda(), lens, out_dtype=F32)
+    fa.copy_pages([c], [P - 1, P - 2], [P - 4, 1])
+    moved = torch.tensor([[P - 4, 5, P - 3], [1, 40000, 33000]], dtype=torch.int32)
+    assert torch.equal(out, fa.paged_attention(q.cuda(), c, moved.cuda(), lens, out_dtype=F32))
+    small = fa.PagedCache(*(t[bt.flatten().long().cuda()].contiguous() for t in (c.k_codes, c.k_scales, c.v)))
+    assert torch.equal(out, fa.paged_attention(q.cuda(), small, torch.arange(6).int().view(2, 3).cuda(), lens, out_dtype=F32))
     assert fa.status_query() == fa.OK
 
 
