@@ -12,8 +12,12 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <climits>
+#include <optional>
+#include <string>
 #include <vector>
 
 #include "../../include/fp4attn.h"
@@ -175,48 +179,102 @@ bool went(int status, const char* name)
     const at::Device device(at::kCUDA, static_cast<at::DeviceIndex>(PyLong_AsLong(index)));   \
     if (PyErr_Occurred()) return nullptr
 
+// x turned into `out` (undefined: a new tensor); throws on a bad argument.
+Tensor rotary(const Tensor& x, const Tensor& table, const std::optional<Tensor>& positions, bool interleaved, bool inverse,
+              Tensor out)
+{
+    TORCH_CHECK_VALUE(x.dim() == 4 && x.is_cuda() && x.stride(3) == 1,
+                      "x must be a [batch, heads, seq, head_dim] CUDA tensor with a contiguous last dimension");
+    const at::Device device = x.device();
+    const at::ScalarType type = x.scalar_type();
+    const int code = code_of(type);
+    TORCH_CHECK_TYPE(code >= 0, "unsupported dtype ", toString(type), "; use float16 or float32");
+    const int64_t B = x.size(0), H = x.size(1), S = x.size(2), D = x.size(3);
+    TORCH_CHECK_VALUE(B <= INT_MAX && H <= INT_MAX && S <= INT_MAX && D <= INT_MAX, "x is too large");
+    TORCH_CHECK_VALUE(table.dim() == 3 && table.size(2) == 2 && table.scalar_type() == at::kFloat && table.device() == device &&
+                          table.is_contiguous(),
+                      "table must be a contiguous float32 [positions, rotary_dim / 2, 2] tensor on ", device.str());
+    TORCH_CHECK_VALUE(2 * table.size(1) <= D, "the table's rotary_dim ", 2 * table.size(1), " exceeds head_dim ", D);
+    const int32_t* at = nullptr;
+    int64_t at_stride = 0;
+    if (positions) {
+        const Tensor& p = *positions;
+        TORCH_CHECK_VALUE(p.scalar_type() == at::kInt && p.device() == device, "positions must be an int32 tensor on ", device.str());
+        const bool each = p.dim() == 2 && p.size(0) == B && p.size(1) == S;
+        TORCH_CHECK_VALUE(each || (p.dim() == 1 && p.size(0) == S), "positions must be [seq] or [batch, seq]");
+        TORCH_CHECK_VALUE(S < 2 || p.stride(-1) == 1, "positions must be contiguous along seq");
+        at = p.const_data_ptr<int32_t>();
+        at_stride = each ? p.stride(0) : 0;
+    }
+    const c10::cuda::CUDAGuard guard(device);
+    if (!out.defined()) out = make(x.sizes(), type, device);
+    else
+        TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == type && out.device() == device && out.stride(3) == 1,
+                          "out must have x's shape, dtype and device, and a contiguous last dimension");
+    const int64_t xs[3] = {x.stride(0), x.stride(1), x.stride(2)}, os[3] = {out.stride(0), out.stride(1), out.stride(2)};
+    const int status = g.rotary(x.const_data_ptr(), out.mutable_data_ptr(), code, B, H, S, D, xs, os, table.const_data_ptr<float>(),
+                                2 * table.size(1), table.size(0), at, at_stride, interleaved, inverse, stream_of(device));
+    if (status != FP4ATTN_OK) {
+        pybind11::gil_scoped_acquire gil;  // (a backward pass runs without it)
+        went(status, "fp4attn_rotary");
+        throw python_error();
+    }
+    return out;
+}
+
+// A tensor or None.
+bool optional_tensor(PyObject* o, const char* name, std::optional<Tensor>* out)
+{
+    if (o == Py_None) return true;
+    const Tensor* t = tensor(o, name);
+    if (t) *out = *t;
+    return t != nullptr;
+}
+
 PyObject* native_rotary(PyObject*, PyObject* const* args, Py_ssize_t argc)
 {
     HANDLE_TH_ERRORS
     ARGS(6, "rotary");  // x, table, positions, interleaved, inverse, out
     TENSOR(x, args[0], "x");
-    REFUSE(x->dim() != 4 || !x->is_cuda() || x->stride(3) != 1,
-           "x must be a [batch, heads, seq, head_dim] CUDA tensor with a contiguous last dimension");
-    const at::Device device = x->device();
-    const at::ScalarType type = x->scalar_type();
-    DTYPE(code, type);
-    const int64_t B = x->size(0), H = x->size(1), S = x->size(2), D = x->size(3);
-    REFUSE(B > INT_MAX || H > INT_MAX || S > INT_MAX || D > INT_MAX, "x is too large");
-    REFUSE(args[1] == Py_None, "table must be a tensor");
-    Angles angles;
-    if (!good_angles(args[1], device, D, &angles)) return nullptr;
-    const int32_t* positions = nullptr;
-    int64_t positions_stride = 0;
-    if (args[2] != Py_None) {
-        TENSOR(p, args[2], "positions");
-        if (!good_index(*p, device, "positions")) return nullptr;
-        if (p->dim() == 2 && p->size(0) == B && p->size(1) == S) positions_stride = p->stride(0);
-        else REFUSE(p->dim() != 1 || p->size(0) != S, "positions must be [seq] or [batch, seq]");
-        REFUSE(S > 1 && p->stride(-1) != 1, "positions must be contiguous along seq");
-        positions = p->const_data_ptr<int32_t>();
+    TENSOR(table, args[1], "table");
+    std::optional<Tensor> positions, out;
+    if (!optional_tensor(args[2], "positions", &positions) || !optional_tensor(args[5], "out", &out)) return nullptr;
+    const Tensor y = rotary(*x, *table, positions, PyObject_IsTrue(args[3]), PyObject_IsTrue(args[4]), out.value_or(Tensor()));
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// The rotation under autograd: the gradient turns back by the same angles, by
+// this same function, so that it can be differentiated in turn.
+struct Rotary : torch::autograd::Function<Rotary> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& table,
+                          const std::optional<Tensor>& positions, bool interleaved, bool inverse)
+    {
+        ctx->save_for_backward({table, positions.value_or(Tensor())});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["inverse"] = inverse;
+        return rotary(x, table, positions, interleaved, inverse, Tensor());
     }
-    const c10::cuda::CUDAGuard guard(device);
-    Tensor out;
-    if (args[5] == Py_None) {
-        out = make(x->sizes(), type, device);
-    } else {
-        TENSOR(o, args[5], "out");
-        REFUSE(o->sizes() != x->sizes() || o->scalar_type() != type || o->device() != device || o->stride(3) != 1,
-               "out must have x's shape, dtype and device, and a contiguous last dimension");
-        out = *o;
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        Tensor dy = grads[0];
+        if (dy.stride(3) != 1) dy = dy.contiguous();
+        const std::optional<Tensor> positions = saved[1].defined() ? std::optional<Tensor>(saved[1]) : std::nullopt;
+        return {apply(dy, saved[0], positions, ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool()),
+                Tensor(), Tensor(), Tensor(), Tensor()};
     }
-    const int64_t xs[3] = {x->stride(0), x->stride(1), x->stride(2)}, os[3] = {out.stride(0), out.stride(1), out.stride(2)};
-    if (!went(g.rotary(x->const_data_ptr(), out.mutable_data_ptr(), code, B, H, S, D, xs, os, angles.table, angles.rotary_dim,
-                       angles.positions, positions, positions_stride, PyObject_IsTrue(args[3]), PyObject_IsTrue(args[4]),
-                       stream_of(device)),
-              "fp4attn_rotary"))
-        return nullptr;
-    return THPVariable_Wrap(out);
+};
+
+PyObject* native_rotary_embedding(PyObject*, PyObject* const* args, Py_ssize_t argc)
+{
+    HANDLE_TH_ERRORS
+    ARGS(4, "rotary_embedding");  // x, table, positions, interleaved
+    TENSOR(x, args[0], "x");
+    TENSOR(table, args[1], "table");
+    std::optional<Tensor> positions;
+    if (!optional_tensor(args[2], "positions", &positions)) return nullptr;
+    return THPVariable_Wrap(Rotary::apply(*x, *table, positions, static_cast<bool>(PyObject_IsTrue(args[3])), false));
     END_HANDLE_TH_ERRORS
 }
 
@@ -433,6 +491,7 @@ PyCFunction as_method(F f)
 PyMethodDef methods[] = {
     {"bind", as_method(native_bind), METH_FASTCALL, nullptr},
     {"rotary", as_method(native_rotary), METH_FASTCALL, nullptr},
+    {"rotary_embedding", as_method(native_rotary_embedding), METH_FASTCALL, nullptr},
     {"cache_append", as_method(native_cache_append), METH_FASTCALL, nullptr},
     {"cache_gather", as_method(native_cache_gather), METH_FASTCALL, nullptr},
     {"attend", as_method(native_attend), METH_FASTCALL, nullptr},

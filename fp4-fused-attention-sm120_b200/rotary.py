@@ -98,38 +98,11 @@ def rotary(x, table, positions=None, interleaved=False, inverse=False, out=None,
         return native.rotary(x, table, positions, interleaved, inverse, out)
 
 
-_ROTARY_FN = None
-
-
-def _autograd_function():
-    global _ROTARY_FN
-    if _ROTARY_FN is None:
-        torch = sv.torch()
-
-        class Rotary(torch.autograd.Function):
-            """y = rotary(x); dx = rotary(dy, inverse=True)."""
-
-            @staticmethod
-            def forward(ctx, x, table, positions, interleaved):
-                ctx.save_for_backward(table, positions)
-                ctx.interleaved = interleaved
-                return rotary(x, table, positions, interleaved)
-
-            @staticmethod
-            def backward(ctx, dy):
-                table, positions = ctx.saved_tensors
-                if dy.stride(3) != 1:
-                    dy = dy.contiguous()
-                return rotary(dy, table, positions, ctx.interleaved, inverse=True), None, None, None
-
-        _ROTARY_FN = Rotary
-    return _ROTARY_FN
-
-
 def rotary_embedding(x, table, positions=None, interleaved=False):
-    """``rotary`` that autograd can differentiate (with respect to x).
+    """``rotary`` that autograd can differentiate (with respect to x, any number
+    of times): the gradient turns back by the same angles.
 
     As with every operation: when a backward pass is captured into a CUDA
     graph, no eager graph of the same leaves may be alive, for autograd would
     wait for the stream of that one, which ends the capture."""
-    return _autograd_function().apply(x, table, positions, interleaved)
+    return sv.native().rotary_embedding(x, table, positions, interleaved)

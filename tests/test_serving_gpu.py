@@ -108,6 +108,12 @@ def test_rotary_gradient(fa, cuda, rot, interleaved):
     got = float((dx.cpu().double() * v.double()).sum())
     big = 2 * ref.EPS32 * float(((x.detach().cpu().abs() + v.abs()).double() * 2 * dy.abs().double()).sum()) * 4
     assert abs((f[0] - f[1]) / 2 - got) <= big
+    # the gradient's gradient: dx = R^T dy is linear in dy
+    w = dy.cuda().requires_grad_()
+    (dx2,) = torch.autograd.grad(fa.rotary_embedding(x, table, pos.cuda(), interleaved), x, w, create_graph=True)
+    assert torch.equal(dx2, dx)
+    (dw,) = torch.autograd.grad(dx2, w, v.cuda())
+    assert torch.equal(dw, fa.rotary(v.cuda(), table, pos.cuda(), interleaved))
     # a broadcast gradient (stride 0) is as its copy
     (d0,) = torch.autograd.grad(fa.rotary_embedding(x, table, pos.cuda(), interleaved).sum(), x)
     assert torch.equal(d0, fa.rotary(torch.ones(B, H, S, D).cuda(), table, pos.cuda(), interleaved, inverse=True))
