@@ -799,6 +799,7 @@ void clear_error() { g_last_error.clear(); }
 int ready() { return device_ready(); }
 int sms() { return device_sms(); }
 unsigned long long timeout_ns() { return wait_timeout_ns(); }
+bool pdl() { return pdl_enabled(); }
 int map3d(CUtensorMap* m, CUtensorMapDataType dt, int elem_bytes, const void* base, uint64_t inner, uint64_t rows,
           uint64_t slices, uint32_t box_inner, uint32_t box_rows, int swizzle_bytes)
 {

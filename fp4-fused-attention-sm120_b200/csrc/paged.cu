@@ -30,6 +30,7 @@ void clear_error();
 int ready();
 int sms();
 unsigned long long timeout_ns();
+bool pdl();
 
 // The serving kernels' error word, read and cleared (for fp4attn_status_query).
 int serving_status()
@@ -154,13 +155,46 @@ bool wide(const void* p, int dtype, std::initializer_list<int64_t> strides)
 // half of it) is a multiple of eight elements.
 bool whole_eights(int rot, int interleaved) { return (interleaved ? rot : rot / 2) % 8 == 0; }
 
-template <typename T>
-void launch_rotary(dim3 grid, cudaStream_t st, const RotaryArgs& a, bool vec, bool inter)
+// Launches a kernel as the programmatic dependent of whatever precedes it in
+// the stream: a step of serving is a chain of kernels of a few microseconds,
+// each of which comes up while the one before drains and waits for its
+// completion (griddepcontrol.wait) before it touches memory.
+template <typename... KArgs, typename... Args>
+int launch_after(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args)
 {
-    if (vec && inter) rotary_kernel<T, true, true><<<grid, 256, 0, st>>>(a);
-    else if (vec) rotary_kernel<T, true, false><<<grid, 256, 0, st>>>(a);
-    else if (inter) rotary_kernel<T, false, true><<<grid, 256, 0, st>>>(a);
-    else rotary_kernel<T, false, false><<<grid, 256, 0, st>>>(a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = host::pdl() ? 1 : 0;
+    PAGED_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
+    return FP4ATTN_OK;
+}
+
+template <typename T>
+int launch_rotary(dim3 grid, cudaStream_t st, const RotaryArgs& a, bool vec, bool inter)
+{
+    if (vec) return launch_after(inter ? rotary_kernel<T, true, true> : rotary_kernel<T, true, false>, grid, 256, 0, st, a);
+    return launch_after(inter ? rotary_kernel<T, false, true> : rotary_kernel<T, false, false>, grid, 256, 0, st, a);
+}
+
+template <typename T>
+int launch_append(dim3 grid, cudaStream_t st, const AppendArgs& a)
+{
+    return launch_after(a.interleaved ? cache_append_kernel<T, true> : cache_append_kernel<T, false>, grid, kAppendThreads, 0, st, a);
+}
+
+template <typename T>
+int launch_gather(dim3 grid, cudaStream_t st, const GatherArgs& a)
+{
+    int rc = FP4ATTN_OK;
+    with_dim(a.c.head_dim, [&](auto d) { rc = launch_after(cache_gather_kernel<T, d.value>, grid, 256, 0, st, a); });
+    return rc;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
@@ -209,23 +243,6 @@ AttentionWorkspace attention_workspace(int group, int head_dim)
     w.o = w.ml + rows * sizeof(float2);
     w.total = w.o + rows * head_dim * sizeof(float);
     return w;
-}
-
-template <typename... KArgs, typename... Args>
-int launch_after(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    PAGED_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
-    return FP4ATTN_OK;
 }
 
 template <typename OutT, int D, int HC>
@@ -304,8 +321,7 @@ int launch_copies(const std::vector<CopyArray>& arrays, const int32_t* src, cons
         for (int p0 = 0; p0 < n; p0 += kPairs) {
             const int m = std::min(kPairs, n - p0);
             for (int i = 0; i < m; i++) a.pairs[i] = make_int2(src[p0 + i], dst[p0 + i]);
-            copy_pages_kernel<kArrays, kPairs><<<dim3(chunks, m), 256, 0, st>>>(a);
-            PAGED_CUDA(cudaGetLastError());
+            if (int rc = launch_after(copy_pages_kernel<kArrays, kPairs>, dim3(chunks, m), 256, 0, st, a)) return rc;
         }
     }
     return FP4ATTN_OK;
@@ -364,10 +380,8 @@ int fp4attn_rotary(const void* x, void* y, int dtype, int batch, int heads, int 
     while (a.heads_per_thread < 4 && work * batch * (heads / (2 * a.heads_per_thread)) >= 148 * 2048) a.heads_per_thread *= 2;
     const dim3 grid(static_cast<unsigned>((work + 255) / 256), (heads + a.heads_per_thread - 1) / a.heads_per_thread, batch);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FP4ATTN_F16) launch_rotary<__half>(grid, st, a, vec, interleaved != 0);
-    else launch_rotary<float>(grid, st, a, vec, interleaved != 0);
-    PAGED_CUDA(cudaGetLastError());
-    return FP4ATTN_OK;
+    return dtype == FP4ATTN_F16 ? launch_rotary<__half>(grid, st, a, vec, interleaved != 0)
+                                : launch_rotary<float>(grid, st, a, vec, interleaved != 0);
 }
 
 int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* V, const void* Q, void* Q_out, int dtype,
@@ -419,19 +433,13 @@ int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* 
         const int at_once = kAppendThreads / units, sets = (2 * a.c.kv_heads + a.q_heads + at_once - 1) / at_once;
         if (sets > 65535) return fail(FP4ATTN_EINVAL, "%d heads are too many", 2 * a.c.kv_heads + a.q_heads);
         const dim3 grid(tokens, sets);
-        if (f16 && a.interleaved) cache_append_kernel<__half, true><<<grid, kAppendThreads, 0, st>>>(a);
-        else if (f16) cache_append_kernel<__half, false><<<grid, kAppendThreads, 0, st>>>(a);
-        else if (a.interleaved) cache_append_kernel<float, true><<<grid, kAppendThreads, 0, st>>>(a);
-        else cache_append_kernel<float, false><<<grid, kAppendThreads, 0, st>>>(a);
+        return f16 ? launch_append<__half>(grid, st, a) : launch_append<float>(grid, st, a);
     } else {
         const int64_t work = static_cast<int64_t>(tokens) * (2 * a.c.kv_heads + a.q_heads) * (a.c.head_dim / 8);
         if ((work + 255) / 256 > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "%d tokens are too many", tokens);
         const unsigned grid = static_cast<unsigned>((work + 255) / 256);
-        if (f16) cache_append_any_kernel<__half><<<grid, 256, 0, st>>>(a);
-        else cache_append_any_kernel<float><<<grid, 256, 0, st>>>(a);
+        return launch_after(f16 ? cache_append_any_kernel<__half> : cache_append_any_kernel<float>, grid, 256, 0, st, a);
     }
-    PAGED_CUDA(cudaGetLastError());
-    return FP4ATTN_OK;
 }
 
 int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table, int64_t table_stride, int seqs,
@@ -455,10 +463,7 @@ int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table,
     const int rows = 256 / (cache->head_dim / 8) * kGatherRows;
     const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(max_length) + rows - 1) / rows), cache->kv_heads, seqs);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FP4ATTN_F16) with_dim(cache->head_dim, [&](auto d) { cache_gather_kernel<__half, d.value><<<grid, 256, 0, st>>>(a); });
-    else with_dim(cache->head_dim, [&](auto d) { cache_gather_kernel<float, d.value><<<grid, 256, 0, st>>>(a); });
-    PAGED_CUDA(cudaGetLastError());
-    return FP4ATTN_OK;
+    return dtype == FP4ATTN_F16 ? launch_gather<__half>(grid, st, a) : launch_gather<float>(grid, st, a);
 }
 
 size_t fp4attn_paged_attention_workspace_size(int batch, int q_heads, int kv_heads, int head_dim)

@@ -148,6 +148,8 @@ constexpr int kAppendThreads = 128;
 template <typename T, bool kInter>
 __global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const __grid_constant__ AppendArgs a)
 {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     const int D = a.c.head_dim, half = a.rot / 2, pairs = kInter ? 0 : half / 8;
     const int units = kInter ? D / 8 : pairs + (D - a.rot) / 8, at_once = kAppendThreads / units;
     const int hs = threadIdx.x / units, u = threadIdx.x % units;
@@ -161,10 +163,10 @@ __global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const 
     uint4 ra[sizeof(T) / 2], rb[sizeof(T) / 2];
     load_raw8(x, ra);
     if (pair) load_raw8(x + half, rb);
-    const int pos = __ldg(a.positions + tok);
+    const int pos = a.positions[tok];
     const bool valid = pos >= 0 && (!a.rot || pos < a.max_positions);
     int page = -1;
-    if (valid && !is_q) page = page_of(a.c, a.t, a.seq_ids ? __ldg(a.seq_ids + tok) : tok, pos);
+    if (valid && !is_q) page = page_of(a.c, a.t, a.seq_ids ? a.seq_ids[tok] : tok, pos);
     if (!valid && pos >= 0 && u == 0 && h == 0) record_index_error(kIndexPosition, pos);
     if (!is_q && page < 0) return;
     const int64_t place = static_cast<int64_t>(is_v ? h - kv : h) * a.c.page_size + (pos & (a.c.page_size - 1));
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const 
         const float4* cs = reinterpret_cast<const float4*>(a.table + static_cast<int64_t>(pos) * half + e0);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float4 f = __ldg(cs + i);
+            const float4 f = cs[i];
             turn(v[2 * i], w[2 * i], f.x, f.y, v[2 * i], w[2 * i]);
             turn(v[2 * i + 1], w[2 * i + 1], f.z, f.w, v[2 * i + 1], w[2 * i + 1]);
         }
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const 
         const float4* cs = reinterpret_cast<const float4*>(a.table + static_cast<int64_t>(pos) * half + e0 / 2);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const float4 f = __ldg(cs + i);
+            const float4 f = cs[i];
             turn(v[4 * i], v[4 * i + 1], f.x, f.y, v[4 * i], v[4 * i + 1]);
             turn(v[4 * i + 2], v[4 * i + 3], f.z, f.w, v[4 * i + 2], v[4 * i + 3]);
         }
@@ -244,6 +246,8 @@ __device__ __forceinline__ void rotated8(const T* row, int e0, const float2* cs,
 template <typename T>
 __global__ void __launch_bounds__(256) cache_append_any_kernel(const __grid_constant__ AppendArgs a)
 {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     const int D = a.c.head_dim, row8 = D / 8;
     const int kv_units = a.c.kv_heads * row8, units = 2 * kv_units + a.q_heads * row8;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -316,12 +320,14 @@ constexpr int kGatherRows = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) cache_gather_kernel(const __grid_constant__ GatherArgs a)
 {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     constexpr int ROW8 = D / 8, ROWS = 256 / ROW8;  // rows of a block at once
     const int tid = threadIdx.x, e0 = tid % ROW8 * 8, r = tid / ROW8;
     if (r >= ROWS) return;
     const int head = blockIdx.y, seq = blockIdx.z;
-    const int start = a.starts ? __ldg(a.starts + seq) : 0;
-    int length = __ldg(a.lengths + seq);
+    const int start = a.starts ? a.starts[seq] : 0;
+    int length = a.lengths[seq];
     if (start < 0 || length < 0 || length > a.max_length) {
         if (blockIdx.x == 0 && head == 0 && tid == 0) record_index_error(kIndexLength, start < 0 ? start : length);
         length = 0;
@@ -344,10 +350,10 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const __grid_constant
         const int page = page_of(a.c, a.t, seq, static_cast<int>(pos));
         if (page < 0) continue;
         const int64_t in_page = static_cast<int64_t>(head) * a.c.page_size + (pos & (a.c.page_size - 1));
-        code[k] = __ldg(reinterpret_cast<const uint32_t*>(a.c.k_codes + page * a.c.k_codes_stride + in_page * (D / 2) + e0 / 2));
-        scale[k] = scale_value(__ldg(a.c.k_scales + page * a.c.k_scales_stride + in_page * (D / 32) + e0 / 32));
-        value[k] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.c.v) + page * a.c.v_stride +
-                                                        (in_page * D + e0) * 2));
+        code[k] = *reinterpret_cast<const uint32_t*>(a.c.k_codes + page * a.c.k_codes_stride + in_page * (D / 2) + e0 / 2);
+        scale[k] = scale_value(a.c.k_scales[page * a.c.k_scales_stride + in_page * (D / 32) + e0 / 32]);
+        value[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.c.v) + page * a.c.v_stride +
+                                                   (in_page * D + e0) * 2);
     }
 #pragma unroll
     for (int k = 0; k < kGatherRows; k++) {
@@ -394,6 +400,8 @@ struct CopyArgs {
 template <int kArrays, int kPairs>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyArgs<kArrays, kPairs> a)
 {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     int i = 0;
     while (i + 1 < a.n_arrays && a.arrays[i + 1].first_chunk <= static_cast<int>(blockIdx.x)) i++;
     const CopyArray& ar = a.arrays[i];

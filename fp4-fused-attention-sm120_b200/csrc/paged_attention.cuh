@@ -147,7 +147,7 @@ struct PagedArgs {
 
 __device__ __forceinline__ int paged_length(const PagedArgs& a, int b)
 {
-    const int len = __ldg(a.seq_lens + b);
+    const int len = a.seq_lens[b];
     const int64_t most = static_cast<int64_t>(a.t.max_pages) << a.c.page_shift;
     return len < 0 ? 0 : len > most ? static_cast<int>(most) : len;
 }
@@ -444,11 +444,11 @@ __global__ void __launch_bounds__(384, 1)
             const int32_t* row = a.t.pages + t.b * a.t.stride + ((t.tile * kPagedTile) >> shift) + lane;
             const int step = kPagedTile >> shift;  // pages of a tile; lane p has the p-th
             int left = lane < step ? (t.len - t.tile * kPagedTile + page - 1) >> shift : 0;  // pages from this tile on
-            int id = lane < left ? __ldg(row) : 0;
+            int id = lane < left ? *row : 0;
             for (int i = 0; i < t.n; i++, g++, ring.next()) {
                 row += step;
                 left -= step;
-                const int next_id = i + 1 < t.n && lane < left ? __ldg(row) : 0;
+                const int next_id = i + 1 < t.n && lane < left ? *row : 0;
                 if (id < 0 || id >= a.c.pages) {
                     record_index_error(kIndexPage, id);
                     id = 0;
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(384, 1)
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(&q_full[wg]);
                 if (row == 127 && t.first_of_sequence()) {
-                    const int len = __ldg(a.seq_lens + t.b);
+                    const int len = a.seq_lens[t.b];
                     if (len != t.len) record_index_error(kIndexLength, len);
                 }
             }
@@ -871,6 +871,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     __shared__ float4 sums[kRows][D / 4];
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, h = blockIdx.y;
     ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     const int4 it = a.p.items[blockIdx.x];
     if (it.x < 0) return;
     const int h0 = (it.y % a.splits) * a.heads_per_group;
@@ -880,7 +881,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     // The first rows of parts are on their way while the weights are formed.
     const int r = tid / (D / 4), c = tid % (D / 4);
     auto part = [&](int p) {
-        return __ldg(reinterpret_cast<const float4*>(a.p.o + (static_cast<int64_t>(slot(p)) * HC + h) * D) + c);
+        return reinterpret_cast<const float4*>(a.p.o + (static_cast<int64_t>(slot(p)) * HC + h) * D)[c];
     };
     float4 first = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < kRows && r < parts) first = part(r);

@@ -109,6 +109,8 @@ struct RotaryArgs {
 template <typename T, bool kVec, bool kInter>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a)
 {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
     constexpr int E = kVec ? 8 : 1;
     const int half = a.rot / 2;
     const int turned = kVec ? (kInter ? a.rot / 8 : half / 8) : half;
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a)
         if constexpr (kVec) {
 #pragma unroll
             for (int i = 0; i < P; i += 2) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(row + i));
+                const float4 f = *reinterpret_cast<const float4*>(row + i);
                 cs[i] = make_float2(f.x, a.sign * f.y);
                 cs[i + 1] = make_float2(f.z, a.sign * f.w);
             }
