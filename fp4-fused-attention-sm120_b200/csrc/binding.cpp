@@ -7,6 +7,7 @@
 // four.  The functions are those of the shared library, by the addresses that
 // the Python side looked up; there is no arithmetic here.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -179,6 +180,16 @@ bool went(int status, const char* name)
     const at::Device device(at::kCUDA, static_cast<at::DeviceIndex>(PyLong_AsLong(index)));   \
     if (PyErr_Occurred()) return nullptr
 
+// Checks `out`, which a call reads `in` to write: it may be `in`, but neither
+// lie half over it nor have elements that share memory.  Its version is moved
+// on, so that autograd notices where it had kept the old contents.
+void writes_over(const Tensor& out, const Tensor& in, const char* name)
+{
+    TORCH_CHECK_VALUE(at::has_internal_overlap(out) != at::MemOverlap::Yes, "elements of out share memory");
+    TORCH_CHECK_VALUE(at::get_overlap_status(in, out) != at::MemOverlapStatus::Partial, "out lies partly over ", name);
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 // x turned into `out` (undefined: a new tensor); throws on a bad argument.
 Tensor rotary(const Tensor& x, const Tensor& table, const std::optional<Tensor>& positions, bool interleaved, bool inverse,
               Tensor out)
@@ -207,10 +218,12 @@ Tensor rotary(const Tensor& x, const Tensor& table, const std::optional<Tensor>&
         at_stride = each ? p.stride(0) : 0;
     }
     const c10::cuda::CUDAGuard guard(device);
-    if (!out.defined()) out = make(x.sizes(), type, device);
+    const bool given = out.defined();
+    if (!given) out = make(x.sizes(), type, device);
     else
         TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == type && out.device() == device && out.stride(3) == 1,
                           "out must have x's shape, dtype and device, and a contiguous last dimension");
+    if (given) writes_over(out, x, "x");
     const int64_t xs[3] = {x.stride(0), x.stride(1), x.stride(2)}, os[3] = {out.stride(0), out.stride(1), out.stride(2)};
     const int status = g.rotary(x.const_data_ptr(), out.mutable_data_ptr(), code, B, H, S, D, xs, os, table.const_data_ptr<float>(),
                                 2 * table.size(1), table.size(0), at, at_stride, interleaved, inverse, stream_of(device));
@@ -274,6 +287,7 @@ PyObject* native_rotary_embedding(PyObject*, PyObject* const* args, Py_ssize_t a
     TENSOR(table, args[1], "table");
     std::optional<Tensor> positions;
     if (!optional_tensor(args[2], "positions", &positions)) return nullptr;
+    REFUSE(table->requires_grad(), "the table has no gradient");
     return THPVariable_Wrap(Rotary::apply(*x, *table, positions, static_cast<bool>(PyObject_IsTrue(args[3])), false));
     END_HANDLE_TH_ERRORS
 }
@@ -318,6 +332,7 @@ PyObject* native_cache_append(PyObject*, PyObject* const* args, Py_ssize_t argc)
         q = Q->const_data_ptr();
         qs[0] = Q->stride(0);
         qs[1] = Q->stride(1);
+        REFUSE(Q->size(1) > INT_MAX, "Q is too large");
         q_heads = static_cast<int>(Q->size(1));
     }
     const long rule = PyLong_AsLong(args[10]);
@@ -401,6 +416,7 @@ PyObject* native_attend(PyObject*, PyObject* const* args, Py_ssize_t argc)
                    (args[7] != Py_None && o->scalar_type() != out_type),
                "out must be contiguous with Q's shape, on its device");
         out = *o;
+        writes_over(out, *Q, "Q");
     }
     DTYPE(out_code, out.scalar_type());
     const bool with_lse = PyObject_IsTrue(args[9]);

@@ -87,6 +87,27 @@ def test_rotary_strides_and_in_place(fa, cuda, interleaved):
     assert torch.equal(fa.rotary(e, table), fa.rotary(e.contiguous(), table))
 
 
+def test_outputs_that_cannot_be_written(fa, cuda):
+    """out= with shared elements or half over the input is refused; out=x moves x's version on."""
+    B, H, S, D = 2, 3, 8, 64
+    table = fa.rotary_table(S, D)
+    base = torch.randn(2 * B * H * S * D, generator=_gen(6)).half().cuda()
+    x = base[:B * H * S * D].view(B, H, S, D)
+    with pytest.raises(ValueError, match="share memory"):
+        fa.rotary(x, table, out=x[:, :1].expand(B, H, S, D))
+    with pytest.raises(ValueError, match="partly"):
+        fa.rotary(x, table, out=base[D:D + B * H * S * D].view(B, H, S, D))
+    beside = base[B * H * S * D:].view(B, H, S, D)
+    assert torch.equal(fa.rotary(x, table, out=beside), fa.rotary(x, table))
+    w = torch.randn(D, generator=_gen(7)).half().cuda().requires_grad_()
+    loss = (x * w).sum()
+    fa.rotary(x, table, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(ValueError, match="no gradient"):
+        fa.rotary_embedding(x, table.clone().requires_grad_())
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("rot", [64, 30])
 def test_rotary_gradient(fa, cuda, rot, interleaved):
@@ -627,6 +648,22 @@ def test_attention_on_two_streams(fa, cuda):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert fa.status_query() == fa.OK
+
+
+def test_attention_writes_over_its_queries(fa, cuda):
+    """out=Q gives the plain call's bytes; an output half over Q is refused."""
+    cache = fa.PagedCache.empty(40, 16, 2, 64)
+    table = torch.arange(40, device="cuda", dtype=torch.int32).view(2, 20)
+    lens = torch.tensor([300, 17], device="cuda", dtype=torch.int32)
+    seq = torch.arange(2, device="cuda", dtype=torch.int32).repeat_interleave(320)
+    K, V = (torch.randn(640, 2, 64, generator=_gen(s)).half().cuda() for s in (8, 9))
+    fa.cache_append(cache, K, V, table, torch.arange(320, device="cuda", dtype=torch.int32).repeat(2), seq_ids=seq)
+    base = torch.randn(3, 4, 64, generator=_gen(10)).half().cuda()
+    want = fa.paged_attention(base[:2].clone(), cache, table, lens)
+    with pytest.raises(ValueError, match="partly"):
+        fa.paged_attention(base[:2], cache, table, lens, out=base[1:])
+    fa.paged_attention(base[:2], cache, table, lens, out=base[:2])
+    assert torch.equal(base[:2], want)
 
 
 def test_attention_refuses_mismatched_tensors(fa, cuda):
