@@ -151,10 +151,6 @@ bool wide(const void* p, int dtype, std::initializer_list<int64_t> strides)
     return true;
 }
 
-// Whether eights of a row are turned whole: the rotated part (halves: each
-// half of it) is a multiple of eight elements.
-bool whole_eights(int rot, int interleaved) { return (interleaved ? rot : rot / 2) % 8 == 0; }
-
 // Launches a kernel as the programmatic dependent of whatever precedes it in
 // the stream: a step of serving is a chain of kernels of a few microseconds,
 // each of which comes up while the one before drains and waits for its
@@ -226,9 +222,9 @@ int encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* b
 }
 
 // Query heads of a group computed at once.  A larger group is split, and its
-// keys and values are read again, from L2: 32 heads at once spilled registers
-// and took as long (144 us for 32 sequences of 1000 to 8000 tokens, 8 x 32 heads of 128;
-// 16 of them 74).
+// keys and values are read again, from L2: for 32 sequences of 1000 to 8000
+// tokens, 8 x 32 query heads of 128, two groups of 16 take 131 us and 32 heads
+// at once, which spilled registers, 144.
 int heads_at_once(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 
 struct AttentionWorkspace {
@@ -371,15 +367,21 @@ int fp4attn_rotary(const void* x, void* y, int dtype, int batch, int heads, int 
     RotaryArgs a{x, y, x_strides[0], x_strides[1], x_strides[2], y_strides[0], y_strides[1], y_strides[2],
                  heads, seq, head_dim, rotary_dim, reinterpret_cast<const float2*>(table), positions, positions_stride,
                  max_positions, inverse ? -1.f : 1.f, 1};
-    const bool vec = whole_eights(rotary_dim, interleaved) && wide(x, dtype, {a.xb, a.xh, a.xs}) &&
-                     wide(y, dtype, {a.yb, a.yh, a.ys});
-    const int64_t turned = vec ? (interleaved ? rotary_dim / 8 : rotary_dim / 16) : rotary_dim / 2;
-    const int64_t work = seq * (turned + (head_dim - rotary_dim) / (vec ? 8 : 1));
+    const bool in_eights = wide(x, dtype, {a.xb, a.xh, a.xs}) && wide(y, dtype, {a.yb, a.yh, a.ys});
+    const bool vec = in_eights && (interleaved || rotary_dim % 16 == 0), by_rows = in_eights && !vec;
+    const int64_t units = by_rows              ? head_dim / 8
+                          : vec && interleaved ? head_dim / 8
+                          : vec                ? rotary_dim / 16 + (head_dim - rotary_dim) / 8
+                                               : head_dim - rotary_dim / 2;
+    const int64_t work = seq * units;
     if (work > 0x7FFFFF00) return fail(FP4ATTN_EINVAL, "seq %d is too long", seq);
     // Several heads a thread where that leaves every SM its 2048 threads.
-    while (a.heads_per_thread < 4 && work * batch * (heads / (2 * a.heads_per_thread)) >= 148 * 2048) a.heads_per_thread *= 2;
-    const dim3 grid(static_cast<unsigned>((work + 255) / 256), (heads + a.heads_per_thread - 1) / a.heads_per_thread, batch);
+    while (a.heads_per_thread < (by_rows ? 16 : 4) && work * batch * (heads / (2 * a.heads_per_thread)) >= 148 * 2048) a.heads_per_thread *= 2;
+    const int64_t blocks = by_rows ? (seq + 256 / units - 1) / (256 / units) : (work + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(blocks), (heads + a.heads_per_thread - 1) / a.heads_per_thread, batch);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (by_rows)
+        return launch_after(dtype == FP4ATTN_F16 ? rotary_rows_kernel<__half> : rotary_rows_kernel<float>, grid, 256, 0, st, a);
     return dtype == FP4ATTN_F16 ? launch_rotary<__half>(grid, st, a, vec, interleaved != 0)
                                 : launch_rotary<float>(grid, st, a, vec, interleaved != 0);
 }
@@ -424,22 +426,22 @@ int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* 
     a.max_positions = max_positions;
     a.interleaved = interleaved != 0;
     a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
-    a.vec = whole_eights(a.rot, a.interleaved) && wide(K, dtype, {a.kt, a.kh}) && wide(V, dtype, {a.vt, a.vh}) &&
-            (!Q || wide(Q, dtype, {a.qt, a.qh}));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = dtype == FP4ATTN_F16;
-    if (a.vec && (a.interleaved || a.rot % 64 == 0)) {
-        const int units = a.interleaved ? a.c.head_dim / 8 : a.rot / 16 + (a.c.head_dim - a.rot) / 8;
+    if (wide(K, dtype, {a.kt, a.kh}) && wide(V, dtype, {a.vt, a.vh}) && (!Q || wide(Q, dtype, {a.qt, a.qh}))) {
+        const bool by_rows = !a.interleaved && a.rot % 64 != 0;
+        const int units = a.interleaved || by_rows ? a.c.head_dim / 8 : a.rot / 16 + (a.c.head_dim - a.rot) / 8;
         const int at_once = kAppendThreads / units, sets = (2 * a.c.kv_heads + a.q_heads + at_once - 1) / at_once;
         if (sets > 65535) return fail(FP4ATTN_EINVAL, "%d heads are too many", 2 * a.c.kv_heads + a.q_heads);
         const dim3 grid(tokens, sets);
+        if (by_rows)
+            return launch_after(f16 ? cache_append_rows_kernel<__half> : cache_append_rows_kernel<float>, grid, kAppendThreads, 0, st, a);
         return f16 ? launch_append<__half>(grid, st, a) : launch_append<float>(grid, st, a);
-    } else {
-        const int64_t work = static_cast<int64_t>(tokens) * (2 * a.c.kv_heads + a.q_heads) * (a.c.head_dim / 8);
-        if ((work + 255) / 256 > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "%d tokens are too many", tokens);
-        const unsigned grid = static_cast<unsigned>((work + 255) / 256);
-        return launch_after(f16 ? cache_append_any_kernel<__half> : cache_append_any_kernel<float>, grid, 256, 0, st, a);
     }
+    const int64_t work = static_cast<int64_t>(tokens) * (2 * a.c.kv_heads + a.q_heads) * (a.c.head_dim / 8);
+    if ((work + 255) / 256 > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "%d tokens are too many", tokens);
+    const unsigned grid = static_cast<unsigned>((work + 255) / 256);
+    return launch_after(f16 ? cache_append_any_kernel<__half> : cache_append_any_kernel<float>, grid, 256, 0, st, a);
 }
 
 int fp4attn_cache_gather(const fp4attn_cache* cache, const int32_t* block_table, int64_t table_stride, int seqs,

@@ -110,7 +110,7 @@ struct PagedCfg {
     // The O^T MMA reads 128 rows (head-dim columns) of V: past head_dim it
     // reads on into what follows; those rows of O^T are not used.
     static constexpr int V_OVER = (MT * 128 - D) / CHE * kPagedTile * CB;
-    static constexpr int MISC = 3072;                                // barriers, reductions
+    static constexpr int MISC = 3 * 1024;                            // barriers, reductions
     static constexpr int kBudget = 227 * 1024 - 1024 - OFF_STAGE - MISC - V_OVER;
     static constexpr int STAGES = kBudget / STAGE < 8 ? kBudget / STAGE : 8;
     static_assert(STAGES >= 2, "shared memory budget exceeded");

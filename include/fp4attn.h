@@ -338,8 +338,8 @@ typedef struct {
  * The codes and scales are byte for byte those of fp4attn_rotary followed by
  * fp4attn_quantize.  No two tokens of a call may have the same place in the
  * cache, and Q_out must not overlap Q.  One block a token in parallel: rows are
- * fastest 16-byte aligned (pointers and strides) with rotary_dim a multiple of
- * 64, or interleaved and a multiple of 8; every other form is taken element by
+ * fastest 16-byte aligned (pointers and strides), with rotary_dim a multiple of
+ * 64 or interleaved pairs; rows that are not aligned are taken element by
  * element. */
 int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* V, const void* Q, void* Q_out,
                          int dtype, int tokens, int q_heads, const int64_t* k_strides, const int64_t* v_strides,

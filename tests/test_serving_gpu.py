@@ -87,6 +87,37 @@ def test_rotary_strides_and_in_place(fa, cuda, interleaved):
     assert torch.equal(fa.rotary(e, table), fa.rotary(e.contiguous(), table))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dim,rot", [(32, 6), (64, 22), (96, 80), (128, 50), (128, 96), (160, 2), (256, 250)])
+def test_rotary_dimensions_across_eights(fa, cuda, dim, rot, interleaved, dtype):
+    """Aligned rows, unaligned rows and the rotation in place give the same bytes, and so does
+    an append of the same rows."""
+    B, H, S = 2, 5, 37
+    table = fa.rotary_table(64, rot)
+    base = torch.randn(B, S, H, dim + 1, generator=_gen(11)).to(dtype).cuda()
+    off = base[..., 1:].transpose(1, 2)  # rows off a 16-byte boundary
+    x = off.contiguous()
+    want = fa.rotary(off, table, interleaved=interleaved)
+    assert torch.equal(fa.rotary(x, table, interleaved=interleaved), want)
+    pages = torch.arange(6, dtype=torch.int32, device="cuda").view(2, 3)
+    pos = torch.arange(S, dtype=torch.int32, device="cuda").repeat(B)
+    seq = torch.arange(B, dtype=torch.int32, device="cuda").repeat_interleave(S)
+    got = []
+    for rows in (x, off):
+        cache = fa.PagedCache.empty(6, 16, H, dim)
+        for t in (cache.k_codes, cache.k_scales, cache.v):
+            t.zero_()
+        r = rows.transpose(1, 2)
+        r = r.reshape(B * S, H, dim) if rows is x else base.view(B * S, H, dim + 1)[..., 1:]
+        q = fa.cache_append(cache, r, r, pages, pos, seq_ids=seq, Q=r, table=table, interleaved=interleaved)
+        assert torch.equal(q, want.transpose(1, 2).reshape(B * S, H, dim))
+        got.append((cache.k_codes, cache.k_scales, cache.v))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    fa.rotary(x, table, interleaved=interleaved, out=x)
+    assert torch.equal(x, want)
+
+
 def test_outputs_that_cannot_be_written(fa, cuda):
     """out= with shared elements or half over the input is refused; out=x moves x's version on."""
     B, H, S, D = 2, 3, 8, 64
