@@ -182,7 +182,10 @@ int launch_rotary(dim3 grid, cudaStream_t st, const RotaryArgs& a, bool vec, boo
 template <typename T>
 int launch_append(dim3 grid, cudaStream_t st, const AppendArgs& a)
 {
-    return launch_after(a.interleaved ? cache_append_kernel<T, true> : cache_append_kernel<T, false>, grid, kAppendThreads, 0, st, a);
+    auto kern = !a.interleaved               ? cache_append_kernel<T, false, false>
+                : a.c.head_dim % 64 == 0 ? cache_append_kernel<T, true, true>
+                                         : cache_append_kernel<T, true, false>;
+    return launch_after(kern, grid, kAppendThreads, 0, st, a);
 }
 
 template <typename T>
@@ -430,7 +433,7 @@ int fp4attn_cache_append(const fp4attn_cache* cache, const void* K, const void* 
     const bool f16 = dtype == FP4ATTN_F16;
     if (wide(K, dtype, {a.kt, a.kh}) && wide(V, dtype, {a.vt, a.vh}) && (!Q || wide(Q, dtype, {a.qt, a.qh}))) {
         const bool by_rows = !a.interleaved && a.rot % 64 != 0;
-        const int units = a.interleaved || by_rows ? a.c.head_dim / 8 : a.rot / 16 + (a.c.head_dim - a.rot) / 8;
+        const int units = by_rows ? a.c.head_dim / 8 : append_units(a.c.head_dim, a.rot, a.interleaved);
         const int at_once = kAppendThreads / units, sets = (2 * a.c.kv_heads + a.q_heads + at_once - 1) / at_once;
         if (sets > 65535) return fail(FP4ATTN_EINVAL, "%d heads are too many", 2 * a.c.kv_heads + a.q_heads);
         const dim3 grid(tokens, sets);

@@ -139,29 +139,62 @@ __device__ __forceinline__ void load_raw8(const float* p, uint4 (&r)[2])
 // for -- the position, then the angles and the page -- is waited for while the
 // row is on its way, once, and 32 registers leave room for all the warps that an
 // SM holds: 17,600 tokens of 32 + 2 x 8 heads of 128 take 95 us, 0.67 of their
-// 63 us at the copy rate.  (With 50 registers 114 us; with three heads a thread,
-// their angles kept, and 78 registers 156.)  Needs 16-byte aligned rows and, for halves, a rotary dimension
-// of whole 64s, so that a block of 32 is four neighbouring lanes'.
+// 63 us at the copy rate.  (With 50 registers 114 us; with three heads a
+// thread, their angles kept, and 78 registers 156; interleaved 101 us, with one
+// eight a thread 137.)  Needs 16-byte aligned rows and, for halves, a rotary
+// dimension of whole 64s, so that a block of 32 is four neighbouring lanes'.
 constexpr int kAppendThreads = 128;
 
-template <typename T, bool kInter>
-__global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const __grid_constant__ AppendArgs a)
+// Threads of a row: two eights each where that leaves whole blocks of 32 to four
+// neighbouring lanes (interleaved: head dimensions of whole 64s).
+__host__ __device__ inline int append_units(int head_dim, int rot, bool interleaved)
+{
+    if (interleaved) return head_dim % 64 == 0 ? head_dim / 16 : head_dim / 8;
+    return rot / 16 + (head_dim - rot) / 8;
+}
+
+// Eight interleaved elements from e0 on, of which those below 2 * half are
+// turned.  cs: the position's angles.
+__device__ __forceinline__ void turn_interleaved(float (&v)[8], const float2* cs, int e0, int half)
+{
+    if (e0 >= 2 * half) return;
+    cs += e0 / 2;
+    if (half % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float4 f = reinterpret_cast<const float4*>(cs)[i];
+            turn(v[4 * i], v[4 * i + 1], f.x, f.y, v[4 * i], v[4 * i + 1]);
+            turn(v[4 * i + 2], v[4 * i + 3], f.z, f.w, v[4 * i + 2], v[4 * i + 3]);
+        }
+    } else {  // the last eight may be turned in part
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (e0 / 2 + i >= half) break;
+            const float2 f = cs[i];
+            turn(v[2 * i], v[2 * i + 1], f.x, f.y, v[2 * i], v[2 * i + 1]);
+        }
+    }
+}
+
+// kTwo: interleaved, two eights a thread (head dimensions of whole 64s).
+template <typename T, bool kInter, bool kTwo>
+__global__ void __launch_bounds__(kAppendThreads, kTwo ? 12 : 16) cache_append_kernel(const __grid_constant__ AppendArgs a)
 {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const int D = a.c.head_dim, half = a.rot / 2, pairs = kInter ? 0 : half / 8;
-    const int units = kInter ? D / 8 : pairs + (D - a.rot) / 8, at_once = kAppendThreads / units;
+    const int D = a.c.head_dim, half = a.rot / 2, units = append_units(D, a.rot, kInter), at_once = kAppendThreads / units;
+    const int second = kInter ? D / 2 : half, pairs = kInter ? D / 16 : half / 8;
     const int hs = threadIdx.x / units, u = threadIdx.x % units;
     const int tok = blockIdx.x, kv = a.c.kv_heads, h = blockIdx.y * at_once + hs;  // K, V, Q
     if (hs >= at_once || h >= 2 * kv + a.q_heads) return;
-    const bool pair = !kInter && u < pairs, is_v = h >= kv && h < 2 * kv, is_q = h >= 2 * kv;
+    const bool pair = (!kInter || kTwo) && u < pairs, is_v = h >= kv && h < 2 * kv, is_q = h >= 2 * kv;
     const int e0 = kInter || pair ? 8 * u : a.rot + 8 * (u - pairs);
     const T* x = (is_q   ? static_cast<const T*>(a.q) + tok * a.qt + (h - 2 * kv) * a.qh
                   : is_v ? static_cast<const T*>(a.v) + tok * a.vt + (h - kv) * a.vh
                          : static_cast<const T*>(a.k) + tok * a.kt + h * a.kh) + e0;
     uint4 ra[sizeof(T) / 2], rb[sizeof(T) / 2];
     load_raw8(x, ra);
-    if (pair) load_raw8(x + half, rb);
+    if (pair) load_raw8(x + second, rb);
     const int pos = a.positions[tok];
     const bool valid = pos >= 0 && (!a.rot || pos < a.max_positions);
     int page = -1;
@@ -173,14 +206,14 @@ __global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const 
         __half* dst = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(a.c.v) + page * a.c.v_stride) + place * D + e0;
         if constexpr (sizeof(T) == 2) {  // FP16 values keep their bits
             *reinterpret_cast<uint4*>(dst) = ra[0];
-            if (pair) *reinterpret_cast<uint4*>(dst + half) = rb[0];
+            if (pair) *reinterpret_cast<uint4*>(dst + second) = rb[0];
         } else {
             float v[8];
             load8v(reinterpret_cast<const T*>(ra), v);
             store8v(dst, v);
             if (pair) {
                 load8v(reinterpret_cast<const T*>(rb), v);
-                store8v(dst + half, v);
+                store8v(dst + second, v);
             }
         }
         return;
@@ -191,6 +224,10 @@ __global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const 
     if (!valid) {  // padding, and angles that are not there: a row of zeros
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = w[i] = 0.f;
+    } else if constexpr (kInter) {
+        const float2* cs = a.table + static_cast<int64_t>(pos) * half;
+        turn_interleaved(v, cs, e0, half);
+        if (pair) turn_interleaved(w, cs, e0 + second, half);
     } else if (pair) {
         const float4* cs = reinterpret_cast<const float4*>(a.table + static_cast<int64_t>(pos) * half + e0);
 #pragma unroll
@@ -199,31 +236,14 @@ __global__ void __launch_bounds__(kAppendThreads, 16) cache_append_kernel(const 
             turn(v[2 * i], w[2 * i], f.x, f.y, v[2 * i], w[2 * i]);
             turn(v[2 * i + 1], w[2 * i + 1], f.z, f.w, v[2 * i + 1], w[2 * i + 1]);
         }
-    } else if (kInter && e0 < a.rot) {
-        const float2* cs = a.table + static_cast<int64_t>(pos) * half + e0 / 2;
-        if (half % 4 == 0) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float4 f = reinterpret_cast<const float4*>(cs)[i];
-                turn(v[4 * i], v[4 * i + 1], f.x, f.y, v[4 * i], v[4 * i + 1]);
-                turn(v[4 * i + 2], v[4 * i + 3], f.z, f.w, v[4 * i + 2], v[4 * i + 3]);
-            }
-        } else {  // a last eight may be turned in part
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (e0 / 2 + i >= half) break;
-                const float2 f = cs[i];
-                turn(v[2 * i], v[2 * i + 1], f.x, f.y, v[2 * i], v[2 * i + 1]);
-            }
-        }
     }
     if (is_q) {
         T* dst = static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.q_heads + h - 2 * kv) * D + e0;
         store8v(dst, v);
-        if (pair) store8v(dst + half, w);
+        if (pair) store8v(dst + second, w);
     } else {
         put_key<T>(a.c, page, place, e0, v, a.ocp);
-        if (pair) put_key<T>(a.c, page, place, e0 + half, w, a.ocp);
+        if (pair) put_key<T>(a.c, page, place, e0 + second, w, a.ocp);
     }
 }
 
