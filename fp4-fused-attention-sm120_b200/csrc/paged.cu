@@ -247,7 +247,7 @@ AttentionWorkspace attention_workspace(int group, int head_dim)
 template <typename OutT, int D, int HC>
 int launch_attention(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
 {
-    using C = PagedCfg<D, HC, sizeof(OutT) == 4>;
+    using C = PagedCfg<D, HC>;
     auto kern = paged_attention_kernel<OutT, D, HC>;
     // The shared memory limit is an attribute of the kernel in a context.
     static std::atomic<unsigned long long> done[64];

@@ -43,13 +43,22 @@
 // of a tile took 3,000 (0.196 ms for 64 sequences of up to 8192 tokens).
 //
 // The softmax reference m starts as the item's first tile's maximum and is
-// moved only when a score exceeds it by more than 2^8 (FP16 P would come near
-// its range at 2^16); all threads hold the same m in registers and agree by
-// one barrier with a vote.  P is rounded to FP16 for FP16 output (2^-11 of
-// each weight, below the rounding of the result); for FP32 output it is split
-// into two FP16 parts, which the same accumulation adds.  Each tile's O^T is
-// added to FP32 registers with proper rounding: only 128 keys are summed
-// inside the tensor core.
+// moved only when a score exceeds it by more than 2^8; all threads hold the
+// same m in registers and agree by one barrier with a vote.  The weights
+// p = 2^(z - m), at most 2^8, enter the MMA as two FP16 parts in columns of
+// their own,
+//     hi = fp16(2^7 p),   lo = fp16(2^11 (2^7 p - hi)),   2^7 p ~ hi + 2^-11 lo,
+// which keep 22 bits of every weight down to 2^-21 of the reference's, and
+// below it lose at most 2^-43 of that: both factors use up FP16's range
+// (2^7 2^8 = 2^15, and half a step there times 2^11 is 2^15 again).  One part,
+// or parts that are not lifted, lose the weights of a long tail behind one
+// dominating key (weights below 2^-25 vanish, while the sum still counts them).
+// The second part costs FP16 output nothing where memory bounds it (113 us
+// for 64 sequences of up to 8192 tokens, 8 x 32 heads of 128, either way) and
+// the softmax's time for groups of 16 small heads (32 sequences of 1000 to 8000
+// tokens, 8 x 128 heads of 64: 61 -> 68 us; of 32: 57 -> 71).
+// Each tile's O^T is added to FP32 registers with proper rounding: only 128
+// keys are summed inside the tensor core.
 #pragma once
 
 #include <cuda.h>
@@ -65,15 +74,17 @@ namespace fp4attn {
 constexpr int kPagedBlocks = 148;
 constexpr int kPagedTile = 128;
 
+constexpr float kLift = 0x1p7f, kLowLift = 0x1p11f;  // the factors of P's parts, see above
+
 // HC: query heads computed (4, 8 or 16, at least the group's share).
-template <int D, int HC, bool kSplitP>
+template <int D, int HC>
 struct PagedCfg {
     static constexpr int THREADS = 384;
     // Tiles a step: the roles wait for one another once a step.  Tiles of
     // small heads are short, so two make a step.
     static constexpr int U = D <= 64 ? 2 : 1;
     static constexpr int NS = 16;                                    // N of the S^T MMA (the least there is)
-    static constexpr int NP = kSplitP && HC == 16 ? 32 : 16;         // N of the O^T MMA: with two parts, low parts from NP / 2 on
+    static constexpr int NP = HC == 16 ? 32 : 16;                    // N of the O^T MMA: the low parts from NP / 2 on
     static constexpr int KROW = D <= 64 ? 32 : D <= 128 ? 64 : 128;  // bytes of a key's codes in shared memory (= swizzle)
     static constexpr int KSTEPS = (D + 63) / 64;                     // mxf4 MMAs of K = 64 per S^T tile
     static constexpr int ATOMS = (KSTEPS + 1) / 2;                   // 512-byte scale atoms (four blocks of 32)
@@ -362,8 +373,7 @@ __global__ void __launch_bounds__(384, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                            const __grid_constant__ PagedArgs a)
 {
-    constexpr bool kSplitP = sizeof(OutT) == 4;
-    using C = PagedCfg<D, HC, kSplitP>;
+    using C = PagedCfg<D, HC>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_MISC);
@@ -745,11 +755,13 @@ __global__ void __launch_bounds__(384, 1)
                             const float p0 = ptx::ex2_approx(x[u][h]), p1 = ptx::ex2_approx(x[u][h + 1]);
                             l[h] += p0;
                             l[h + 1] += p1;
-                            hi[h / 2] = ptx::pack_half2(p0, p1);
-                            if constexpr (kSplitP) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[h / 2]));
-                                lo[h / 2] = ptx::pack_half2(p0 - f.x, p1 - f.y);
-                            }
+                            const float2 p = make_float2(p0, p1), lifted = ptx::fmul2(p, make_float2(kLift, kLift));
+                            hi[h / 2] = ptx::pack_half2(lifted.x, lifted.y);
+                            // 2^11 (2^7 p - hi), which is exact
+                            const float2 rest = ptx::ffma2(__half22float2(*reinterpret_cast<const __half2*>(&hi[h / 2])),
+                                                           make_float2(-kLowLift, -kLowLift),
+                                                           ptx::fmul2(p, make_float2(kLift * kLowLift, kLift * kLowLift)));
+                            lo[h / 2] = ptx::pack_half2(rest.x, rest.y);
                         }
                         uint8_t* p = smem + C::OFF_P + (buf * C::U + u) * C::P_BYTES + row * C::PROW;
                         const int sw = C::PROW == 32 ? (row >> 2) & 1 : (row >> 1) & 3;
@@ -764,7 +776,7 @@ __global__ void __launch_bounds__(384, 1)
                             }
                         };
                         put(0, hi);
-                        if constexpr (kSplitP) put(C::NP / 2, lo);
+                        put(C::NP / 2, lo);
                         const int keys = t.keys(i * C::U + u);
                         if (keys % 16 != 0 || keys == 0) {
                             // Keys behind the last, up to the end of its MMA step:
@@ -786,23 +798,27 @@ __global__ void __launch_bounds__(384, 1)
                     ok = bounded_wait(&o_full[buf], static_cast<uint32_t>(done / 2) & 1u, w, kPagedOFull) && ok;
                     __syncwarp();
                     ptx::tc_fence_after();
-                    uint32_t r[C::MT][HC], r2[C::MT][HC];
+                    // (One M at a time: two of 16 heads at once spilled registers.)
 #pragma unroll
                     for (int m = 0; m < C::MT; m++) {
-                        load_cols(C::O_COL + (buf * C::MT + m) * C::NP, r[m]);
-                        if constexpr (kSplitP) load_cols(C::O_COL + (buf * C::MT + m) * C::NP + C::NP / 2, r2[m]);
-                    }
-                    ptx::tc_wait_ld();
-                    ptx::tc_fence_before();
-                    ptx::mbar_arrive(&o_free[buf]);
-#pragma unroll
-                    for (int m = 0; m < C::MT; m++)
-#pragma unroll
-                        for (int h = 0; h < HC; h++) {
-                            float v = __uint_as_float(r[m][h]);
-                            if constexpr (kSplitP) v += __uint_as_float(r2[m][h]);
-                            o[m][h] = fmaf(v, beta[h], o[m][h]);
+                        uint32_t hi[HC], lo[HC];
+                        load_cols(C::O_COL + (buf * C::MT + m) * C::NP, hi);
+                        load_cols(C::O_COL + (buf * C::MT + m) * C::NP + C::NP / 2, lo);
+                        ptx::tc_wait_ld();
+                        if (m == C::MT - 1) {
+                            ptx::tc_fence_before();
+                            ptx::mbar_arrive(&o_free[buf]);
                         }
+#pragma unroll
+                        for (int h = 0; h < HC; h += 2) {
+                            const float2 v = ptx::ffma2(make_float2(__uint_as_float(lo[h]), __uint_as_float(lo[h + 1])),
+                                                        make_float2(1.f / kLowLift, 1.f / kLowLift),
+                                                        make_float2(__uint_as_float(hi[h]), __uint_as_float(hi[h + 1])));
+                            const float2 sum = ptx::ffma2(v, make_float2(beta[h], beta[h + 1]), make_float2(o[m][h], o[m][h + 1]));
+                            o[m][h] = sum.x;
+                            o[m][h + 1] = sum.y;
+                        }
+                    }
                 }
             }
             if (out_of_time) break;
@@ -823,7 +839,7 @@ __global__ void __launch_bounds__(384, 1)
                 if (h >= nh) break;
                 const float sum = (red_sum[h] + red_sum[HC + h]) + (red_sum[2 * HC + h] + red_sum[3 * HC + h]);
                 if (whole) {
-                    const float inv = sum > 0.f ? __fdividef(1.0f, sum) : 0.f;
+                    const float inv = sum > 0.f ? __fdividef(1.f / kLift, sum) : 0.f;
 #pragma unroll
                     for (int m = 0; m < C::MT; m++)
                         if (m * 128 + row < D)
@@ -834,7 +850,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
                     for (int m = 0; m < C::MT; m++)
                         if (m * 128 + row < D)
-                            a.p.o[(static_cast<int64_t>(slot) * HC + h) * D + m * 128 + row] = o[m][h];
+                            a.p.o[(static_cast<int64_t>(slot) * HC + h) * D + m * 128 + row] = o[m][h] * (1.f / kLift);
                     if (row == h) a.p.ml[slot * HC + h] = make_float2(-nm[h], sum);
                 }
             }

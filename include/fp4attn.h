@@ -369,8 +369,9 @@ size_t fp4attn_paged_attention_workspace_size(int batch, int q_heads, int kv_hea
  * lse (or null): [batch, q_heads] natural log-sum-exp.  A sequence of length
  * 0 gives zeros and +inf.  Several new tokens of one sequence are as many
  * rows that share its pages, with lengths that grow by one.
- * softmax_scale <= 0 selects 1/sqrt(head_dim).  FP16 output: the probabilities
- * are rounded to FP16 once, as in the forward; FP32 output: they keep 22 bits.
+ * softmax_scale <= 0 selects 1/sqrt(head_dim).  With either output type the
+ * probabilities keep 22 bits down to 2^-21 of the largest, and those below lose
+ * at most 2^-43 of it; FP16 output is the FP32 output rounded once.
  * A length beyond the block table counts as the table's, and a page outside the
  * cache as page 0 (FP4ATTN_EINDEX either way; the other sequences keep their
  * results).  max_pages * page_size is at most 2^30.  Results repeat bit for bit
