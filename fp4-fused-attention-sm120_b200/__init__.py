@@ -23,6 +23,7 @@ __all__ = [
     "fp4_attention_backward", "FP4Attention", "fp4_attention", "selftest_backward_abort",
     "rotary_frequencies", "rotary_table", "rotary", "rotary_embedding", "PagedCache", "cache_append", "cache_gather",
     "paged_attention_workspace_size", "paged_attention", "paged_attention_lse", "copy_pages", "PagePool",
+    "selftest_paged_abort",
 ]
 
 BLOCK_ELEMENT = 32  # common.h:15
@@ -412,6 +413,18 @@ def selftest_backward_abort(Q, K, V, out, dout, lse, dq, dk, dv, workspace, time
                                                  dv.data_ptr(), B, H, Sq, Sk, workspace.data_ptr(), workspace.numel(),
                                                  timeout_us, _stream_ptr(stream)),
            "fp4attn_selftest_backward_abort")
+    return status_query(stream)
+
+
+def selftest_paged_abort(Q, cache, block_table, seq_lens, out, workspace, timeout_us: int = 20000, stream=None) -> int:
+    """Run paged attention's abort self-test (fp4attn_selftest_paged_abort) over
+    a head_dim-64 cache, FP16 Q and float32 out; returns status_query()
+    (FP4ATTN_ETIMEOUT when the failure path ran)."""
+    _check(lib().fp4attn_selftest_paged_abort(ctypes.byref(cache.struct), Q.data_ptr(), out.data_ptr(), Q.shape[0],
+                                              Q.shape[1], block_table.data_ptr(), block_table.stride(0),
+                                              block_table.shape[1], seq_lens.data_ptr(), workspace.data_ptr(),
+                                              workspace.numel(), timeout_us, _stream_ptr(stream)),
+           "fp4attn_selftest_paged_abort")
     return status_query(stream)
 
 

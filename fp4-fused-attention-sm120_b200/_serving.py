@@ -27,8 +27,10 @@ def declare(L) -> None:
     L.fp4attn_cache_gather.argtypes = [cache, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, i32, vp]
     L.fp4attn_paged_attention_workspace_size.argtypes = [i32] * 4
     L.fp4attn_paged_attention.argtypes = ([cache, vp, vp, vp] + [i32] * 4 + [vp, vp, i64, i32, vp, f32, i32, vp, sz, vp])
+    L.fp4attn_selftest_paged_abort.argtypes = [cache, vp, vp, i32, i32, vp, i64, i32, vp, vp, sz, ctypes.c_uint, vp]
     L.fp4attn_copy_pages.argtypes = [cache, i32, vp, vp, i32, vp]
-    for name in ("rotary_table", "rotary", "cache_append", "cache_gather", "paged_attention", "copy_pages"):
+    for name in ("rotary_table", "rotary", "cache_append", "cache_gather", "paged_attention", "copy_pages",
+                 "selftest_paged_abort"):
         getattr(L, "fp4attn_" + name).restype = i32
     L.fp4attn_paged_attention_workspace_size.restype = sz
 

@@ -244,11 +244,11 @@ AttentionWorkspace attention_workspace(int group, int head_dim)
     return w;
 }
 
-template <typename OutT, int D, int HC>
+template <typename OutT, int D, int HC, bool kWithhold = false>
 int launch_attention(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
 {
     using C = PagedCfg<D, HC>;
-    auto kern = paged_attention_kernel<OutT, D, HC>;
+    auto kern = paged_attention_kernel<OutT, D, HC, kWithhold>;
     // The shared memory limit is an attribute of the kernel in a context.
     static std::atomic<unsigned long long> done[64];
     int dev = 0;
@@ -303,6 +303,71 @@ int launch_dim(const PagedArgs& a, int blocks, bool join, cudaStream_t st)
         case 160: return launch_heads<OutT, 160>(a, blocks, join, st);
         default: return launch_heads<OutT, 256>(a, blocks, join, st);
     }
+}
+
+// fp4attn_paged_attention.  test_timeout_ns > 0: its abort self-test, the FP32
+// output kernel of up to four heads of 64 with one withheld arrival, waits
+// bounded by that time.
+int do_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out, float* lse, int in_dtype, int out_dtype, int batch,
+                       int q_heads, const int64_t* q_strides, const int32_t* block_table, int64_t table_stride, int max_pages,
+                       const int32_t* seq_lens, float softmax_scale, int scale_mode, void* workspace, size_t workspace_bytes,
+                       void* stream, unsigned long long test_timeout_ns = 0)
+{
+    if (int rc = check_cache(cache)) return rc;
+    if (bad_dtype(in_dtype) || bad_dtype(out_dtype)) return fail(FP4ATTN_EINVAL, "dtype %d, %d", in_dtype, out_dtype);
+    if (scale_mode != FP4ATTN_SCALE_REFERENCE && scale_mode != FP4ATTN_SCALE_OCP)
+        return fail(FP4ATTN_EINVAL, "scale_mode %d", scale_mode);
+    if (batch < 0 || batch > 65535) return fail(FP4ATTN_EINVAL, "batch %d in [0, 65535]", batch);
+    if (q_heads < 1 || q_heads % cache->kv_heads)
+        return fail(FP4ATTN_EINVAL, "q_heads %d is not a multiple of kv_heads %d", q_heads, cache->kv_heads);
+    if (int rc = check_table(block_table, table_stride, batch, max_pages)) return rc;
+    // (the device counts tokens and tiles in 32 bits)
+    if (static_cast<int64_t>(max_pages) * cache->page_size > (1 << 30))
+        return fail(FP4ATTN_EINVAL, "max_pages %d of %d tokens: more than 2^30", max_pages, cache->page_size);
+    const int64_t longest = (static_cast<int64_t>(max_pages) * cache->page_size + kPagedTile - 1) / kPagedTile;
+    const int64_t most_tiles = longest * q_heads * batch;
+    if (most_tiles > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "batch %d x heads %d x max_pages %d: more than 2^31 tiles", batch, q_heads, max_pages);
+    if (batch == 0) return FP4ATTN_OK;
+    if (!Q || !Out || !q_strides || !seq_lens) return fail(FP4ATTN_EINVAL, "null pointer");
+    if (!wide(Q, in_dtype, {q_strides[0], q_strides[1]}) || !aligned(Out, 16) || !aligned(lse, 4) || !aligned(seq_lens, 4) ||
+        !aligned(block_table, 4))
+        return fail(FP4ATTN_EINVAL, "Q (and its strides) and Out must be 16-byte aligned");
+    const size_t need = fp4attn_paged_attention_workspace_size(batch, q_heads, cache->kv_heads, cache->head_dim);
+    if (!workspace || workspace_bytes < need)
+        return fail(FP4ATTN_EWORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
+    if (!aligned(workspace, 256)) return fail(FP4ATTN_EINVAL, "workspace must be 256-byte aligned");
+    if (int rc = host::ready()) return rc;
+    PagedArgs a{};
+    a.q = Q;
+    a.q_half = in_dtype == FP4ATTN_F16;
+    a.qb = q_strides[0];
+    a.qh = q_strides[1];
+    a.batch = batch;
+    a.q_heads = q_heads;
+    a.group = q_heads / cache->kv_heads;
+    a.c = view_of(*cache);
+    a.t = TableView{block_table, table_stride, batch, max_pages};
+    a.seq_lens = seq_lens;
+    const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(cache->head_dim));
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
+    a.out = Out;
+    a.lse = lse;
+    const int nh = heads_at_once(a.group);
+    a.splits = (a.group + nh - 1) / nh;
+    a.heads_per_group = (a.group + a.splits - 1) / a.splits;
+    a.head_groups = cache->kv_heads * a.splits;
+    const AttentionWorkspace ws = attention_workspace(a.group, cache->head_dim);
+    char* base = static_cast<char*>(workspace);
+    a.p = PagedPartials{reinterpret_cast<float*>(base + ws.o), reinterpret_cast<float2*>(base + ws.ml),
+                        reinterpret_cast<int4*>(base + ws.items)};
+    a.timeout_ns = test_timeout_ns ? test_timeout_ns : host::timeout_ns();
+    // The most tiles the block table allows; what there are is known on the device.
+    const int64_t tiles = longest * a.head_groups * batch;
+    const int blocks = static_cast<int>(std::min<int64_t>({kPagedBlocks, host::sms(), tiles}));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (test_timeout_ns) return launch_attention<float, 64, 4, true>(a, blocks, longest > 1, st);
+    return out_dtype == FP4ATTN_F16 ? launch_dim<__half>(a, blocks, longest > 1, st) : launch_dim<float>(a, blocks, longest > 1, st);
 }
 
 template <int kArrays, int kPairs>
@@ -483,60 +548,23 @@ int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out
                             int scale_mode, void* workspace, size_t workspace_bytes, void* stream)
 {
     host::clear_error();
+    return do_paged_attention(cache, Q, Out, lse, in_dtype, out_dtype, batch, q_heads, q_strides, block_table, table_stride,
+                              max_pages, seq_lens, softmax_scale, scale_mode, workspace, workspace_bytes, stream);
+}
+
+int fp4attn_selftest_paged_abort(const fp4attn_cache* cache, const void* Q, float* Out, int batch, int q_heads,
+                                 const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
+                                 void* workspace, size_t workspace_bytes, unsigned timeout_us, void* stream)
+{
+    host::clear_error();
+    if (timeout_us < 1 || timeout_us > 10000000u) return fail(FP4ATTN_EINVAL, "timeout_us in [1, 1e7]");
     if (int rc = check_cache(cache)) return rc;
-    if (bad_dtype(in_dtype) || bad_dtype(out_dtype)) return fail(FP4ATTN_EINVAL, "dtype %d, %d", in_dtype, out_dtype);
-    if (scale_mode != FP4ATTN_SCALE_REFERENCE && scale_mode != FP4ATTN_SCALE_OCP)
-        return fail(FP4ATTN_EINVAL, "scale_mode %d", scale_mode);
-    if (batch < 0 || batch > 65535) return fail(FP4ATTN_EINVAL, "batch %d in [0, 65535]", batch);
-    if (q_heads < 1 || q_heads % cache->kv_heads)
-        return fail(FP4ATTN_EINVAL, "q_heads %d is not a multiple of kv_heads %d", q_heads, cache->kv_heads);
-    if (int rc = check_table(block_table, table_stride, batch, max_pages)) return rc;
-    // (the device counts tokens and tiles in 32 bits)
-    if (static_cast<int64_t>(max_pages) * cache->page_size > (1 << 30))
-        return fail(FP4ATTN_EINVAL, "max_pages %d of %d tokens: more than 2^30", max_pages, cache->page_size);
-    const int64_t longest = (static_cast<int64_t>(max_pages) * cache->page_size + kPagedTile - 1) / kPagedTile;
-    const int64_t most_tiles = longest * q_heads * batch;
-    if (most_tiles > 0x7FFFFFFF) return fail(FP4ATTN_EINVAL, "batch %d x heads %d x max_pages %d: more than 2^31 tiles", batch, q_heads, max_pages);
-    if (batch == 0) return FP4ATTN_OK;
-    if (!Q || !Out || !q_strides || !seq_lens) return fail(FP4ATTN_EINVAL, "null pointer");
-    if (!wide(Q, in_dtype, {q_strides[0], q_strides[1]}) || !aligned(Out, 16) || !aligned(lse, 4) || !aligned(seq_lens, 4) ||
-        !aligned(block_table, 4))
-        return fail(FP4ATTN_EINVAL, "Q (and its strides) and Out must be 16-byte aligned");
-    const size_t need = fp4attn_paged_attention_workspace_size(batch, q_heads, cache->kv_heads, cache->head_dim);
-    if (!workspace || workspace_bytes < need)
-        return fail(FP4ATTN_EWORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
-    if (!aligned(workspace, 256)) return fail(FP4ATTN_EINVAL, "workspace must be 256-byte aligned");
-    if (int rc = host::ready()) return rc;
-    PagedArgs a{};
-    a.q = Q;
-    a.q_half = in_dtype == FP4ATTN_F16;
-    a.qb = q_strides[0];
-    a.qh = q_strides[1];
-    a.batch = batch;
-    a.q_heads = q_heads;
-    a.group = q_heads / cache->kv_heads;
-    a.c = view_of(*cache);
-    a.t = TableView{block_table, table_stride, batch, max_pages};
-    a.seq_lens = seq_lens;
-    const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(cache->head_dim));
-    a.scale_log2 = scale * 1.4426950408889634f;
-    a.ocp = scale_mode == FP4ATTN_SCALE_OCP;
-    a.out = Out;
-    a.lse = lse;
-    const int nh = heads_at_once(a.group);
-    a.splits = (a.group + nh - 1) / nh;
-    a.heads_per_group = (a.group + a.splits - 1) / a.splits;
-    a.head_groups = cache->kv_heads * a.splits;
-    const AttentionWorkspace ws = attention_workspace(a.group, cache->head_dim);
-    char* base = static_cast<char*>(workspace);
-    a.p = PagedPartials{reinterpret_cast<float*>(base + ws.o), reinterpret_cast<float2*>(base + ws.ml),
-                        reinterpret_cast<int4*>(base + ws.items)};
-    a.timeout_ns = host::timeout_ns();
-    // The most tiles the block table allows; what there are is known on the device.
-    const int64_t tiles = longest * a.head_groups * batch;
-    const int blocks = static_cast<int>(std::min<int64_t>({kPagedBlocks, host::sms(), tiles}));
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return out_dtype == FP4ATTN_F16 ? launch_dim<__half>(a, blocks, longest > 1, st) : launch_dim<float>(a, blocks, longest > 1, st);
+    if (cache->head_dim != 64 || q_heads > 4 * static_cast<int64_t>(cache->kv_heads))
+        return fail(FP4ATTN_EINVAL, "the self-test takes head_dim 64 and up to four query heads a key/value head");
+    const int64_t strides[2] = {64 * static_cast<int64_t>(q_heads), 64};
+    return do_paged_attention(cache, Q, Out, nullptr, FP4ATTN_F16, FP4ATTN_F32, batch, q_heads, strides, block_table, table_stride,
+                              max_pages, seq_lens, 0.f, FP4ATTN_SCALE_REFERENCE, workspace, workspace_bytes, stream,
+                              static_cast<unsigned long long>(timeout_us) * 1000ull);
 }
 
 int fp4attn_copy_pages(const fp4attn_cache* caches, int n_caches, const int32_t* src, const int32_t* dst, int n, void* stream)

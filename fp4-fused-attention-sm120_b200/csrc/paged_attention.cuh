@@ -368,7 +368,9 @@ __device__ __forceinline__ void each_page(int n, const int (&id)[8], F copy)
     if (n & 1) copy(last, last == 0 ? id[0] : last == 2 ? id[2] : last == 4 ? id[4] : id[6]);
 }
 
-template <typename OutT, int D, int HC>
+// kWithhold (test instantiation only, fp4attn_selftest_paged_abort): one thread
+// of block 0 never reports its first weights, so the O^T issuer's wait runs out.
+template <typename OutT, int D, int HC, bool kWithhold = false>
 __global__ void __launch_bounds__(384, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                            const __grid_constant__ PagedArgs a)
@@ -430,6 +432,9 @@ __global__ void __launch_bounds__(384, 1)
     // Everything before this overlaps the grid before this one in the stream.
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
+    // Nothing to join, until this block's last item says otherwise: the join reads
+    // this word even when a wait here runs out and the items are not finished.
+    if (threadIdx.x == 0) a.p.items[blockIdx.x] = make_int4(-1, 0, 0, 0);
     find_range(a, range, scratch);
     ptx::tc_fence_before();
     __syncthreads();
@@ -789,7 +794,7 @@ __global__ void __launch_bounds__(384, 1)
                     }
                     __syncwarp();
                     ptx::fence_proxy_async_smem();
-                    ptx::mbar_arrive(&p_full[buf]);
+                    if (!kWithhold || blockIdx.x > 0 || g > 0 || row > 0) ptx::mbar_arrive(&p_full[buf]);
                     g++;
                     j++;
                 }
@@ -854,15 +859,12 @@ __global__ void __launch_bounds__(384, 1)
                     if (row == h) a.p.ml[slot * HC + h] = make_float2(-nm[h], sum);
                 }
             }
-            if (row == 0 && t.left == t.n) {
-                // What the join has to do for this block: the item begun here that goes on.
-                int4 it = make_int4(-1, 0, 0, 0);
-                if (begun && !whole)  // (to the block of its last tile)
-                    it = make_int4(t.b, t.head * a.splits + t.split, paged_block(range->total, range->first + count - t.n + t.tiles - 1, range->blocks), slot);
-                a.p.items[blockIdx.x] = it;
-            }
+            // What the join has to do for this block: the item begun here that goes on, to
+            // the block of its last tile.
+            if (row == 0 && t.left == t.n && begun && !whole)
+                a.p.items[blockIdx.x] = make_int4(t.b, t.head * a.splits + t.split,
+                                                  paged_block(range->total, range->first + count - t.n + t.tiles - 1, range->blocks), slot);
         }
-        if (count == 0 && threadIdx.x == 128) a.p.items[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
 
     ptx::tc_fence_before();

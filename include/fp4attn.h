@@ -385,6 +385,20 @@ int fp4attn_paged_attention(const fp4attn_cache* cache, const void* Q, void* Out
                             float softmax_scale, int scale_mode, void* workspace, size_t workspace_bytes,
                             void* stream);
 
+/* Test hook for paged attention's failure path (the counterpart of
+ * fp4attn_selftest_abort): the head_dim 64, FP32-output kernel in a build in
+ * which one thread of its first block never reports its first weights, every
+ * wait bounded by timeout_us.  That wait runs out, the block's roles leave their
+ * loops and drain what is in flight, and the join joins what there is:
+ * nothing outside Out and the workspace is written, fp4attn_status_query
+ * reports FP4ATTN_ETIMEOUT, and the sequences of that block hold no result.
+ * Q: [batch, q_heads, 64] FP16, contiguous; at most four query heads a
+ * key/value head; with a first sequence of 640 tokens a block and more the block
+ * leaves in mid-sequence. */
+int fp4attn_selftest_paged_abort(const fp4attn_cache* cache, const void* Q, float* Out, int batch, int q_heads,
+                                 const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
+                                 void* workspace, size_t workspace_bytes, unsigned timeout_us, void* stream);
+
 /* Copies whole pages, src[i] to dst[i], within each of n_caches caches (the
  * layers of a model share one page numbering).  src, dst: host memory, read
  * before the call returns.  A page may be copied to several, but none is
