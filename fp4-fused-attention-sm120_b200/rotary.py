@@ -51,7 +51,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
             return rotary_dim * math.log(original_positions / (times * 2 * math.pi)) / (2 * math.log(base))
 
         low = max(math.floor(pair_that_turns(beta_fast)), 0)
-        high = min(math.ceil(pair_that_turns(beta_slow)), half - 1)
+        high = min(math.ceil(pair_that_turns(beta_slow)), rotary_dim - 1)  # (may lie behind the last pair)
         high = max(high, low + 0.001)
         out = []
         for j, f in enumerate(freqs):
