@@ -7,7 +7,6 @@
 // four.  The functions are those of the shared library, by the addresses that
 // the Python side looked up; there is no arithmetic here.
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -16,6 +15,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
 #include <optional>
 #include <string>
@@ -180,13 +180,69 @@ bool went(int status, const char* name)
     const at::Device device(at::kCUDA, static_cast<at::DeviceIndex>(PyLong_AsLong(index)));   \
     if (PyErr_Occurred()) return nullptr
 
-// Checks `out`, which a call reads `in` to write: it may be `in`, but neither
-// lie half over it nor have elements that share memory.  Its version is moved
-// on, so that autograd notices where it had kept the old contents.
+// One multiple of a stride, least to most, out of a sum of them.
+struct Term {
+    int64_t stride, least, most;
+};
+
+// Whether start + sum_k m_k stride_k can lie between lo and hi (both excluded)
+// for m_k in [least, most], not all of them zero if `moved`.  Strides in falling
+// order, positive; with those of an ordinary view few multiples of each come into
+// question.  A search that takes too long counts as yes.
+bool meets(const std::vector<Term>& t, size_t k, int64_t start, int64_t lo, int64_t hi, bool moved, int& steps)
+{
+    if (++steps > 20000) return true;
+    if (k == t.size()) return !moved && lo < start && start < hi;
+    int64_t below = 0, above = 0;  // what the terms behind this one reach
+    for (size_t i = k + 1; i < t.size(); i++) {
+        below += t[i].least * t[i].stride;
+        above += t[i].most * t[i].stride;
+    }
+    const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t first = std::max(t[k].least, floor_div(lo - above - start, t[k].stride) + 1);
+    const int64_t last = std::min(t[k].most, -floor_div(start + below - hi, t[k].stride) - 1);
+    for (int64_t m = first; m <= last; m++)
+        if (meets(t, k + 1, start + m * t[k].stride, lo, hi, moved && m == 0, steps)) return true;
+    return false;
+}
+
+bool meets(std::vector<Term>& t, int64_t start, int64_t lo, int64_t hi, bool moved)
+{
+    std::sort(t.begin(), t.end(), [](const Term& a, const Term& b) { return a.stride > b.stride; });
+    int steps = 0;
+    return meets(t, 0, start, lo, hi, moved, steps);
+}
+
+// Checks `out`, which a call reads `in` to write, of one shape and both with
+// contiguous rows: it may be `in` or lie between its rows, but neither have
+// elements in common with it otherwise nor with itself.  (Both are mostly slices
+// of a wider projection, so this is decided from the strides.)  Its version is
+// moved on, so that autograd notices where it had kept the old contents.
 void writes_over(const Tensor& out, const Tensor& in, const char* name)
 {
-    TORCH_CHECK_VALUE(at::has_internal_overlap(out) != at::MemOverlap::Yes, "elements of out share memory");
-    TORCH_CHECK_VALUE(at::get_overlap_status(in, out) != at::MemOverlapStatus::Partial, "out lies partly over ", name);
+    const int64_t rows = out.dim() - 1, oe = out.element_size(), ie = in.element_size();
+    if (out.numel() > 0) {
+        std::vector<Term> self, both;
+        bool in_place = out.const_data_ptr() == in.const_data_ptr() && oe == ie;
+        for (int64_t k = 0; k < rows; k++) {
+            const int64_t n = out.size(k), os = out.stride(k) * oe, is = in.stride(k) * ie;
+            if (n == 1) continue;
+            TORCH_CHECK_VALUE(os > 0, "elements of out share memory");
+            self.push_back({os, 1 - n, n - 1});
+            in_place = in_place && os == is;
+            if (os == is) {
+                both.push_back({os, 1 - n, n - 1});
+            } else {
+                both.push_back({os, 0, n - 1});
+                if (is > 0) both.push_back({is, 1 - n, 0});
+            }
+        }
+        const int64_t out_row = out.size(rows) * oe, in_row = in.size(rows) * ie;
+        TORCH_CHECK_VALUE(!meets(self, 0, -out_row, out_row, true), "elements of out share memory");
+        const int64_t apart = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out.const_data_ptr()) -
+                                                   reinterpret_cast<uintptr_t>(in.const_data_ptr()));
+        TORCH_CHECK_VALUE(in_place || !meets(both, apart, -out_row, in_row, false), "out lies partly over ", name);
+    }
     if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
 }
 

@@ -86,7 +86,8 @@ def rotary_table(max_positions, rotary_dim, base=10000.0, scaling=None, factor=1
 def rotary(x, table, positions=None, interleaved=False, inverse=False, out=None, stream=None):
     """x [batch, heads, seq, head_dim] (float16 or float32, any strides with
     the last dimension contiguous) turned by its positions into ``out``
-    (contiguous by default; ``out=x`` turns in place).
+    (contiguous by default; ``out=x`` turns in place, and any other ``out`` may
+    share no element with x).
 
     positions: int32 [seq] or [batch, seq], by default 0 .. seq - 1.
     interleaved: pairs (2j, 2j + 1) instead of (j, j + rotary_dim / 2).
