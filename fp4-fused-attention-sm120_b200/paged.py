@@ -12,6 +12,7 @@ free; copy_pages does the copying.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 from . import _serving as sv
 
@@ -29,7 +30,9 @@ class PagedCache:
     v        float16 [pages, kv_heads, page_size, head_dim]
 
     Each page is contiguous; pages may be apart (a view of one layer of a
-    larger tensor).  The tensors need not be initialised."""
+    larger tensor).  The tensors need not be initialised.  The calls go by the
+    addresses that the tensors had here, so the cache keeps that memory, and its
+    attributes are read-only: another tensor is another PagedCache."""
 
     def __init__(self, k_codes, k_scales, v):
         torch = sv.torch()
@@ -49,14 +52,19 @@ class PagedCache:
                 raise ValueError(f"{name} and its page stride must be 16-byte aligned")
             if P > 1 and t.stride(0) < t[0].numel():
                 raise ValueError(f"pages of {name} overlap")
-        self.k_codes, self.k_scales, self.v = k_codes, k_scales, v
-        self.pages, self.kv_heads, self.page_size, self.head_dim = P, H, S, D
-        self.device = v.device
-        self.struct = sv.CacheStruct(k_codes.data_ptr(), k_scales.data_ptr(), v.data_ptr(),
-                                     max(k_codes.stride(0), k_codes[0].numel()),
-                                     max(k_scales.stride(0), k_scales[0].numel()),
-                                     2 * max(v.stride(0), v[0].numel()), P, S, H, D)
-        self._at = ctypes.addressof(self.struct)
+        # (Aliases, which hold the memory whatever becomes of the caller's tensors.)
+        self._k_codes, self._k_scales, self._v = k_codes.detach(), k_scales.detach(), v.detach()
+        self._pages, self._kv_heads, self._page_size, self._head_dim = P, H, S, D
+        self._device, self._index = v.device, v.device.index
+        self._struct = sv.CacheStruct(k_codes.data_ptr(), k_scales.data_ptr(), v.data_ptr(),
+                                      max(k_codes.stride(0), k_codes[0].numel()),
+                                      max(k_scales.stride(0), k_scales[0].numel()),
+                                      2 * max(v.stride(0), v[0].numel()), P, S, H, D)
+        self._at = ctypes.addressof(self._struct)
+
+    k_codes, k_scales, v, pages, kv_heads, page_size, head_dim, device, struct = (
+        property(operator.attrgetter("_" + name)) for name in
+        ("k_codes", "k_scales", "v", "pages", "kv_heads", "page_size", "head_dim", "device", "struct"))
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, device="cuda"):
@@ -77,11 +85,11 @@ def cache_append(cache, K, V, block_table, positions, seq_ids=None, Q=None, tabl
     rotated by their positions first.  With Q [tokens, heads, head_dim] returns
     the queries rotated the same way, contiguous.  No two tokens of a call may
     have the same place in the cache."""
-    args = (cache._at, cache.device.index, K, V, block_table, positions, seq_ids, Q, table, interleaved,
+    args = (cache._at, cache._index, K, V, block_table, positions, seq_ids, Q, table, interleaved,
             sv.scale_mode(scale_mode))
     if stream is None:
         return sv.native().cache_append(*args)
-    with sv.on(cache.device, stream):
+    with sv.on(cache._device, stream):
         return sv.native().cache_append(*args)
 
 
@@ -91,10 +99,10 @@ def cache_gather(cache, block_table, starts, lengths, max_length, heads=None, dt
     behind them (fp4attn_cache_gather).  starts=None reads from token 0; heads
     (default: the cache's) repeats each key/value head for its query heads, as
     fused_fp4_attention wants them."""
-    args = (cache._at, cache.device.index, block_table, starts, lengths, max_length, heads, dtype)
+    args = (cache._at, cache._index, block_table, starts, lengths, max_length, heads, dtype)
     if stream is None:
         return sv.native().cache_gather(*args)
-    with sv.on(cache.device, stream):
+    with sv.on(cache._device, stream):
         return sv.native().cache_gather(*args)
 
 
@@ -105,11 +113,11 @@ def paged_attention_workspace_size(cache, batch, heads):
 
 
 def _attend(Q, cache, block_table, seq_lens, softmax_scale, scale_mode, out_dtype, out, with_lse, workspace, stream):
-    args = (Q, cache._at, cache.device.index, block_table, seq_lens, softmax_scale, sv.scale_mode(scale_mode),
+    args = (Q, cache._at, cache._index, block_table, seq_lens, softmax_scale, sv.scale_mode(scale_mode),
             out_dtype, out, with_lse, workspace)
     if stream is None:
         return sv.native().attend(*args)
-    with sv.on(cache.device, stream):
+    with sv.on(cache._device, stream):
         return sv.native().attend(*args)
 
 
@@ -144,8 +152,8 @@ def copy_pages(caches, src, dst, stream=None):
     caches = list(caches)
     if not caches:
         return
-    device = caches[0].device
-    if any(c.device != device for c in caches):
+    device = caches[0]._device
+    if any(c._device != device for c in caches):
         raise ValueError("the caches must be on one device")
     args = ([c._at for c in caches], device.index, _page_numbers(src, "src"), _page_numbers(dst, "dst"))
     if stream is None:

@@ -1,0 +1,38 @@
+"""The handles of serving: a cache's memory stays the memory that its calls go by."""
+import gc
+
+import pytest
+import torch
+
+FIELDS = ("k_codes", "k_scales", "v", "pages", "kv_heads", "page_size", "head_dim", "device", "struct")
+
+
+@pytest.mark.parametrize("name", FIELDS)
+def test_a_cache_is_read_only(fa, name):
+    cache = fa.PagedCache.__new__(fa.PagedCache)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, None)
+    with pytest.raises(AttributeError):
+        delattr(cache, name)
+
+
+@pytest.mark.gpu
+def test_a_cache_keeps_its_memory(fa, cuda):
+    """Neither the caller's tensors nor their replacement take the memory away from the calls."""
+    codes = torch.zeros(4, 1, 16, 32, dtype=torch.uint8, device="cuda")
+    scales = torch.full((4, 1, 16, 2), 127, dtype=torch.uint8, device="cuda")
+    v = torch.zeros(4, 1, 16, 64, dtype=torch.float16, device="cuda")
+    cache = fa.PagedCache(codes, scales, v)
+    at = [t.data_ptr() for t in (cache.k_codes, cache.k_scales, cache.v)]
+    v.data = torch.ones_like(v)
+    del codes, scales
+    gc.collect()
+    new = [torch.full((4, 1, 16, 64), 3.0, dtype=torch.float16, device="cuda") for _ in range(8)]
+    assert not {t.data_ptr() for t in new} & set(at)
+    x = torch.full((1, 1, 64), 2.0, dtype=torch.float16, device="cuda")
+    page, first = torch.tensor([[2]], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    fa.cache_append(cache, x, x, page, first)
+    assert at == [t.data_ptr() for t in (cache.k_codes, cache.k_scales, cache.v)]
+    assert bool((cache.v[2, 0, 0] == 2).all()) and bool((v == 1).all()) and all(bool((t == 3).all()) for t in new)
+    assert bool((fa.paged_attention(x, cache, page, first + 1) == 2).all())
+    assert fa.status_query() == fa.OK
