@@ -145,6 +145,10 @@ bool good_angles(PyObject* o, const at::Device& d, int64_t head_dim, Angles* out
                      static_cast<long long>(head_dim));
         return false;
     }
+    if (t->numel() == 0) {  // (a null pointer would read as no table at all)
+        PyErr_SetString(PyExc_ValueError, "the table is empty");
+        return false;
+    }
     *out = Angles{t->const_data_ptr<float>(), static_cast<int>(2 * t->size(1)), t->size(0)};
     return true;
 }

@@ -36,3 +36,18 @@ def test_a_cache_keeps_its_memory(fa, cuda):
     assert bool((cache.v[2, 0, 0] == 2).all()) and bool((v == 1).all()) and all(bool((t == 3).all()) for t in new)
     assert bool((fa.paged_attention(x, cache, page, first + 1) == 2).all())
     assert fa.status_query() == fa.OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 32, 2), (8, 0, 2)])
+def test_an_empty_rotary_table_is_not_none(fa, cuda, shape):
+    """Keys are not stored unrotated where a table was asked for."""
+    cache = fa.PagedCache.empty(2, 16, 1, 64)
+    cache.v.zero_()
+    x = torch.ones(1, 1, 64, dtype=torch.float16, device="cuda")
+    page, first = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="empty"):
+        fa.cache_append(cache, x, x, page, first, Q=x, table=torch.empty(shape, device="cuda"))
+    with pytest.raises((ValueError, fa.Fp4AttnError)):
+        fa.rotary(x[None], torch.empty(shape, device="cuda"))
+    assert not cache.v.any() and fa.status_query() == fa.OK
