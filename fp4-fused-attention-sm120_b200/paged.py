@@ -166,10 +166,12 @@ def _page_numbers(pages, name):
     """A contiguous int32 CPU tensor of page numbers (their range is checked by the library)."""
     torch = sv.torch()
     if not isinstance(pages, torch.Tensor):
-        pages = torch.tensor(pages, dtype=torch.int64)
-    if pages.dtype is torch.int64 and not pages.is_cuda:
+        pages = torch.tensor(pages) if len(pages) else torch.empty(0, dtype=torch.int64)
+    if pages.dtype is not torch.int32 and not pages.is_cuda:
+        if pages.is_floating_point() or pages.is_complex() or pages.dtype is torch.bool:
+            raise TypeError(f"{name}: page numbers must be integers, not {pages.dtype}")
         narrow = pages.to(torch.int32)
-        if not torch.equal(narrow.to(torch.int64), pages):
+        if not torch.equal(narrow.to(torch.int64), pages.to(torch.int64)):
             raise ValueError(f"{name}: page number out of range")
         pages = narrow
     return pages.contiguous()

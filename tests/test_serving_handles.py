@@ -51,3 +51,20 @@ def test_an_empty_rotary_table_is_not_none(fa, cuda, shape):
     with pytest.raises((ValueError, fa.Fp4AttnError)):
         fa.rotary(x[None], torch.empty(shape, device="cuda"))
     assert not cache.v.any() and fa.status_query() == fa.OK
+
+
+def test_page_numbers_are_integers(fa):
+    """Of any integer type and as lists; fractions and truth values are not cut to page 0."""
+    from fp4attn_b200 import paged
+    for t in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
+        got = paged._page_numbers(torch.tensor([3, 0, 7], dtype=t), "src")
+        assert got.dtype == torch.int32 and got.tolist() == [3, 0, 7]
+    assert paged._page_numbers([5, 1], "src").tolist() == [5, 1]
+    assert paged._page_numbers(range(3), "src").tolist() == [0, 1, 2]
+    assert paged._page_numbers([], "src").shape == (0,)
+    for bad in ([0.7], [1.0, 2.0], [True], torch.tensor([0.0])):
+        with pytest.raises(TypeError, match="src"):
+            paged._page_numbers(bad, "src")
+    for bad in ([2 ** 31], [2 ** 32], torch.tensor([-2 ** 31 - 1])):
+        with pytest.raises(ValueError, match="src"):
+            paged._page_numbers(bad, "src")
