@@ -293,4 +293,4 @@ class PagePool:
         if pages < longest:
             raise ValueError(f"a sequence has {longest} pages, more than {pages}")
         rows = [self._tables[s] + [0] * (pages - len(self._tables[s])) for s in seqs]
-        return torch.tensor(rows, dtype=torch.int32).reshape(len(seqs), pages).to(device or "cpu")
+        return torch.tensor(rows, dtype=torch.int32).reshape(len(seqs), pages).to("cpu" if device is None else device)

@@ -68,3 +68,14 @@ def test_page_numbers_are_integers(fa):
     for bad in ([2 ** 31], [2 ** 32], torch.tensor([-2 ** 31 - 1])):
         with pytest.raises(ValueError, match="src"):
             paged._page_numbers(bad, "src")
+
+
+@pytest.mark.gpu
+def test_block_tables_on_a_device_by_its_number(fa, cuda):
+    pool = fa.PagePool(8, 16)
+    seq = pool.new()
+    pool.extend(seq, 20)
+    for device in (0, "cuda", "cuda:0", torch.device("cuda", 0)):
+        t = pool.block_table([seq], device=device)
+        assert t.device == torch.device("cuda", 0) and t.tolist() == [pool.table(seq)]
+    assert pool.block_table([seq]).device.type == "cpu"
