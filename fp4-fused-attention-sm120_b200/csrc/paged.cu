@@ -226,8 +226,8 @@ int encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* b
 
 // Query heads of a group computed at once.  A larger group is split, and its
 // keys and values are read again, from L2: for 32 sequences of 1000 to 8000
-// tokens, 8 x 32 query heads of 128, two groups of 16 take 131 us and 32 heads
-// at once, which spilled registers, 144.
+// tokens, 8 x 32 query heads of 128, two groups of 16 take 129 us; 32 heads at
+// once, which spilled registers, took 144 when two groups took 131.
 int heads_at_once(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 
 struct AttentionWorkspace {
